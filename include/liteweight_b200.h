@@ -40,7 +40,8 @@ typedef enum {
   LW_ERR_UNSUPPORTED = 5,    /* valid input the library does not handle */
   LW_ERR_LAUNCH = 6,         /* the CUDA launch failed (cudaGetLastError) */
   LW_ERR_WORKSPACE = 7,      /* workspace missing or too small */
-  LW_ERR_TIMEOUT = 8         /* a bounded device-side wait gave up */
+  LW_ERR_TIMEOUT = 8,        /* a bounded device-side wait gave up */
+  LW_ERR_BAD_INDEX = 9       /* a page id, position or length on the device is out of range (that access was skipped) */
 } lw_status;
 
 /* Human-readable name of a status code (static string). */
@@ -55,7 +56,9 @@ unsigned long long lw_launch_count(void);
 
 /* Reads and clears the library's device-side error flags on the current
  * device: LW_ERR_TIMEOUT if a bounded wait inside one of its kernels gave up
- * since the last call (that launch's results are invalid), else LW_OK.
+ * since the last call (that launch's results are invalid), LW_ERR_BAD_INDEX if
+ * a paged-cache kernel skipped an access because a page id, a position or a
+ * length was out of range, else LW_OK.
  * Synchronises the device. No counterpart in the reference. */
 int lw_take_device_error(void);
 
@@ -279,8 +282,9 @@ int lw_attention_decode(const lw_attention_args* args, lw_stream_t stream);
 
 /* sizeof(lw_fused_gemv_args) for which = 0, sizeof(lw_attention_args) for
  * which = 1, sizeof(lw_exchange_out) for 2, sizeof(lw_exchange_in) for 3,
- * sizeof(lw_prefill_gemm_args) for 4, else 0: lets a binding check its
- * struct layouts at load time. */
+ * sizeof(lw_prefill_gemm_args) for 4, sizeof(lw_paged_cache) for 5,
+ * sizeof(lw_qk_norm_rope_args) for 6, sizeof(lw_paged_attention_args) for 7,
+ * else 0: lets a binding check its struct layouts at load time. */
 size_t lw_struct_size(int which);
 
 /* x[b] = embed[tokens[*pos][b]] (tokens int32 [max_seq+1][batch]). */
@@ -381,6 +385,104 @@ int lw_rmsnorm_rows(const void* x, const void* gamma, void* h, int M, int K, flo
  * (modeling_llama.py:63-68 and the residual add of :290-335). */
 int lw_resid_rmsnorm_rows(void* x, const float* psum, const void* gamma, void* h, int M, int K, float eps, int pdl,
                           lw_stream_t stream);
+
+/* ---- paged key-value cache (no counterpart in the reference, whose KVCache,
+ * liteweight/generate.py:7-46, keeps one contiguous block per layer) ----
+ *
+ * Token t of sequence b lives in slot t % page_size of page
+ * page_table[b][t / page_size]. kv_lens[b] counts the sequence's tokens with
+ * the newest ones. A table entry that no visible token needs is not read, so
+ * it may hold anything. Page ids outside [0, n_pages), lengths past
+ * table_width * page_size and positions past the rotation table are skipped
+ * and recorded (lw_take_device_error: LW_ERR_BAD_INDEX): such a key counts as
+ * hidden, such a new token is not stored.
+ *
+ * q_offsets [batch + 1] (device, q_offsets[0] = 0, never falling): rows
+ * q_offsets[b] .. q_offsets[b + 1] - 1 are the newest tokens of sequence b, the
+ * last of them at position kv_lens[b] - 1. Rows from q_offsets[batch] on belong
+ * to no sequence: left as they were, or zeroed with zero_tail.
+ *
+ * Strides are in elements and multiples of 8; the last dimension is contiguous;
+ * pointers are 16-byte aligned. dtype: LW_DTYPE_F16 or LW_DTYPE_BF16 of q, k,
+ * v, the pools, the norm weights and the outputs.
+ */
+enum { LW_DTYPE_F16 = 0, LW_DTYPE_BF16 = 1, LW_DTYPE_F32 = 2 };
+
+typedef struct {
+  void* k_pages;             /* [n_pages][n_kv_heads][page_size][head_dim], any order by the strides */
+  void* v_pages;
+  long long k_strides[3];    /* page, head, slot */
+  long long v_strides[3];
+  int n_pages, page_size;    /* page_size: a power of two, 16 .. 256 */
+  int n_kv_heads, head_dim;  /* head_dim 64 or 128 */
+  int dtype;
+  int batch;                 /* sequences */
+  const int* page_table;     /* int32 [batch][table_width], rows table_stride apart */
+  long long table_stride;
+  int table_width;
+  const int* kv_lens;        /* int32 [batch] */
+} lw_paged_cache;
+
+/* Norms of queries and keys for each head, the rotation by position and the
+ * append of K and V to the cache, in one pass:
+ *   y = x * rsqrt(mean(x^2) + eps) * weight     (weight NULL: y = x)
+ *   o[d] = y[d] * cos[p][d] + r[d] * sin[p][d],  r = (-y[hd/2:], y[:hd/2])
+ * in fp32 with one rounding at the end (cos / sin as modeling_llama.py:124-136
+ * lays them out, [rope_rows][head_dim], fp32 or dtype). Row t is a token of the
+ * sequence q_offsets names, or of sequence t when q_offsets is NULL
+ * (tokens == batch, one new token each; kv_lens[t] = 0: a row of no sequence).
+ * q_out may be q itself. No two new tokens may share a slot. */
+typedef struct {
+  lw_paged_cache cache;
+  const void *q, *k, *v;         /* [tokens][heads][head_dim] */
+  long long q_strides[2], k_strides[2], v_strides[2];   /* token, head */
+  void* q_out;
+  long long out_strides[2];
+  int tokens, n_q_heads;
+  const int* q_offsets;
+  const void *rope_cos, *rope_sin;
+  long long rope_stride;         /* elements between positions */
+  int rope_dtype, rope_rows;
+  const void *q_weight, *k_weight;   /* [head_dim], or both NULL */
+  float eps;
+  int zero_tail;
+  int pdl;
+} lw_qk_norm_rope_args;
+
+int lw_qk_norm_rope(const lw_qk_norm_rope_args* args, lw_stream_t stream);
+
+/* Attention over the paged cache: position p of sequence b sees key j when
+ * j <= p and (window <= 0, or p - j < window, or j < sinks);
+ *   out = sum_j softmax_j(scale * q.k_j) v_j,
+ * zero where no key is visible. Keys outside the mask never reach a result,
+ * whatever they hold. Scores, softmax and sums in fp32; the softmax weights are
+ * rounded to dtype for the second product.
+ *
+ * q_offsets NULL: one new token per sequence (tokens == batch), the cache's
+ * length split over the GPU and joined; else prompt chunks. n_q_heads is a
+ * multiple of n_kv_heads (prompt chunks: at most 64 times).
+ *
+ * workspace: lw_paged_attention_workspace_size() bytes of device scratch, 256
+ * byte aligned, that no other call in flight uses; its contents do not matter
+ * before and after. */
+typedef struct {
+  lw_paged_cache cache;
+  const void* q;
+  long long q_strides[2];        /* token, head */
+  void* out;
+  long long out_strides[2];
+  int tokens, n_q_heads;
+  const int* q_offsets;
+  int window, sinks;
+  float scale;
+  int zero_tail;
+  int pdl;
+  void* workspace;
+  size_t workspace_bytes;
+} lw_paged_attention_args;
+
+int lw_paged_attention(const lw_paged_attention_args* args, lw_stream_t stream);
+size_t lw_paged_attention_workspace_size(const lw_paged_attention_args* args);
 
 /* ---- peer memory for the exchanges (setup calls: these allocate, map and
  * synchronise; they are not stream-ordered and must not be graph-captured) */

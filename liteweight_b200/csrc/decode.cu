@@ -855,6 +855,9 @@ size_t lw_struct_size(int which) {
   if (which == 2) return sizeof(lw_exchange_out);
   if (which == 3) return sizeof(lw_exchange_in);
   if (which == 4) return sizeof(lw_prefill_gemm_args);
+  if (which == 5) return sizeof(lw_paged_cache);
+  if (which == 6) return sizeof(lw_qk_norm_rope_args);
+  if (which == 7) return sizeof(lw_paged_attention_args);
   return 0;
 }
 

@@ -392,6 +392,9 @@ cudaError_t launch_kn(GemvParams p, cudaStream_t s) {
 int lw_decode_take_error();
 int lw_decode_tp_take_error();
 int lw_gemm_tc_take_error();
+int lw_paged_rope_take_error();
+int lw_paged_decode_take_error();
+int lw_paged_prompt_take_error();
 
 extern "C" {
 
@@ -406,18 +409,24 @@ const char* lw_status_string(int status) {
     case LW_ERR_LAUNCH: return "CUDA launch failed";
     case LW_ERR_WORKSPACE: return "workspace missing or too small";
     case LW_ERR_TIMEOUT: return "device wait timed out";
+    case LW_ERR_BAD_INDEX: return "page id, position or length out of range";
     default: return "unknown status";
   }
 }
 
-int lw_abi_version(void) { return 113; }
+int lw_abi_version(void) { return 114; }
 
 int lw_take_device_error(void) {
   const int mine = lw_tu_take_error();
   const int dec = lw_decode_take_error();
   const int tp = lw_decode_tp_take_error();
   const int tc = lw_gemm_tc_take_error();
-  return mine ? mine : (dec ? dec : (tp ? tp : tc));
+  const int rope = lw_paged_rope_take_error();
+  const int pdec = lw_paged_decode_take_error();
+  const int pprm = lw_paged_prompt_take_error();
+  for (int e : {mine, dec, tp, tc, pprm, pdec, rope})
+    if (e) return e;
+  return LW_OK;
 }
 
 unsigned long long lw_launch_count(void) { return g_launches.load(std::memory_order_relaxed); }

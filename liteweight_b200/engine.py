@@ -36,6 +36,7 @@ from dataclasses import dataclass
 import torch
 
 from liteweight_b200 import _native as nat
+from liteweight_b200.kernels import paged
 
 c_int, c_void_p, c_float, c_size_t = ctypes.c_int, ctypes.c_void_p, ctypes.c_float, ctypes.c_size_t
 
@@ -142,7 +143,8 @@ def check_abi() -> None:
     """The ctypes mirrors must have the library's struct sizes."""
     lib = nat.lib()
     for which, cls in ((0, FusedGemvArgs), (1, AttentionArgs), (2, ExchangeOut), (3, ExchangeIn),
-                       (4, PrefillGemmArgs)):
+                       (4, PrefillGemmArgs), (5, paged.PagedCacheArgs), (6, paged.QkNormRopeArgs),
+                       (7, paged.PagedAttentionArgs)):
         got = int(lib.lw_struct_size(which))
         if got != ctypes.sizeof(cls):
             raise RuntimeError(f"{cls.__name__}: ctypes size {ctypes.sizeof(cls)} != library size {got}")
