@@ -460,7 +460,7 @@ int lw_qk_norm_rope(const lw_qk_norm_rope_args* args, lw_stream_t stream);
  *
  * q_offsets NULL: one new token per sequence (tokens == batch), the cache's
  * length split over the GPU and joined; else prompt chunks. n_q_heads is a
- * multiple of n_kv_heads (prompt chunks: at most 64 times).
+ * multiple of n_kv_heads (prompt chunks: at most 64 times); scale > 0.
  *
  * workspace: lw_paged_attention_workspace_size() bytes of device scratch, 256
  * byte aligned, that no other call in flight uses; its contents do not matter

@@ -2,266 +2,523 @@
 // q_offsets): the newest tokens of every sequence against all it keeps, causal,
 // with an optional window and first keys that stay visible.
 //
-// A CTA takes a tile of 64 rows = consecutive positions x the query heads of
-// one kv head's group, so K and V are read once for the whole group, and
-// walks the 64-key tiles any of its rows sees. S = Q K^T and O += P V with
-// mma.sync, online softmax in fp32 per row.
+//   S = scale Q K^T, P = exp2(S log2(e) - m), O = sum P V / sum P
 //
-// Keys that no row of the tile sees are zero-filled by the copy. A key that
-// some rows see and others do not (the diagonal, the window's edge) meets the
-// other rows with weight 0; if its value holds an infinity or a NaN, 0 * v would
-// reach them, so the values of such tiles are scanned, non-finite ones are
-// replaced by 0 and added afterwards to the rows that see them.
+// on the 5th-generation tensor cores. A CTA (one per SM) takes two tiles of 128
+// rows; a row is a position x a query head of one kv head's group, so K and V
+// are read once for the group and a tile spans only 128 / group positions (few
+// masked keys on the diagonal and at a window's edges). It walks the 128-key
+// tiles that any of its rows sees. Tensor memory holds, for each of the two row
+// tiles, S (128 fp32 columns; P in 16 bits overwrites its first 64) and O
+// (head_dim fp32 columns). The ten warps are specialised:
+//   warps 0-3, 4-7  softmax of row tile 0 / 1, one row per thread: read S, mask,
+//                   keep the running maximum and sum in fp32, write P. The
+//                   accumulator is rescaled only when a row's maximum has grown
+//                   by more than 2^8 (P stays below 256, exact in range; the
+//                   sum and O carry the same factor), so O rarely moves.
+//   warp 8          TMA copies: Q once, K and V tiles page by page into a ring.
+//   warp 9          issues tcgen05.mma: S_g = Q_g K^T (both from shared memory),
+//                   O_g += P_g V (P from tensor memory). While one row tile is in
+//                   its softmax the tensor cores work on the other.
+// tcgen05.mma instructions of one thread run in the order they are issued, so S of
+// the next keys may overwrite P as soon as the product that reads P is issued,
+// and the barrier of S(j) covers O's update j - 1 too.
+//
+// When the row tiles alone leave SMs idle (few rows, a long cache) the keys are
+// cut into slices as well; each writes (m, sum, fp32 O) to the workspace and a
+// second kernel joins them in order.
+//
+// What hidden slots hold never reaches a result. Pages that no row sees are
+// zero-filled by the copy (their table entries are not read). In a tile that
+// some row does not see whole, the values are scanned: rows of V that nobody
+// sees are cleared, and where a value that some rows see is an infinity or a NaN
+// it is cleared too (0 * it would reach the others) and added at the end to the
+// rows that see it.
+//
+// Every wait is bounded; on expiry LW_ERR_TIMEOUT is recorded and the CTA ends.
+#include <algorithm>
+
 #include "paged.cuh"
+#include "tcgen05.cuh"
+#include "tma_host.cuh"
 
 namespace lw {
 
+constexpr int kPmRows = 128;                 // rows per tile (UMMA M)
+constexpr int kPmKeys = 128;                 // keys per tile
+constexpr int kPmThreads = 320;
+constexpr int kPmTmaWarp = 8, kPmMmaWarp = 9;
+constexpr long long kPmWaitNs = 2000000000;
+constexpr float kPmGrow = 8.0f;              // log2 of the largest P
+
 struct PromptParams {
+  CUtensorMap tm_q;   // {head_dim, heads, tokens}, box {64, group, rp}
+  CUtensorMap tm_k;   // {head_dim, slots, kv heads, pages}, box {64, min(page, 128), 1, 1}
+  CUtensorMap tm_v;
   PagedView c;
-  const void* q;
   void* out;
-  long long q_t, q_h, o_t, o_h;
+  long long o_t, o_h;
   int T, nq, group, rp;   // rp: positions per row tile
+  int no_page;            // a page index past the pool: its copy is zeros
   const int* off;
   int window, sinks;
   float scale_log2;
   int zero_tail;
+  int slices;
+  float2* part_ml;        // [slices][T][nq]
+  float* part_o;          // [slices][T][nq][head_dim]
 };
 
-// Row tiles of the ragged batch: sequence b owns the slots from off[b] / rp + b
-// on, at least as many as its rows need (ceil(n / rp) <= floor((off + n) / rp) -
-// floor(off / rp) + 1), so a slot finds its sequence by bisection and the grid
-// needs only T and B. Slots without rows exit.
+// Row tiles of the ragged batch: sequence b owns the slots from off[b] / R + b
+// on (R positions per CTA), at least as many as its rows need (ceil(n / R) <=
+// floor((off + n) / R) - floor(off / R) + 1), so a slot finds its sequence by
+// bisection and the grid needs only T and B. Slots without rows exit.
 LW_DEV bool find_row_tile(const PromptParams& p, int slot, int& b, int& i0, int& n) {
+  const int R = 2 * p.rp;
   int lo = 0, hi = p.c.B;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (p.off[mid] / p.rp + mid <= slot) lo = mid;
+    if (p.off[mid] / R + mid <= slot) lo = mid;
     else hi = mid;
   }
   b = lo;
   const int o = p.off[b];
   n = p.off[b + 1] - o;
-  i0 = (slot - (o / p.rp + b)) * p.rp;
+  i0 = (slot - (o / R + b)) * R;
   return i0 >= 0 && i0 < n && o >= 0 && (long long)o + n <= p.T;
 }
 
-constexpr int kPmRows = 64, kPmKeys = 64, kPmThreads = 128;
+LW_DEV float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <int HD>
+struct PromptSmem {
+  static constexpr int kTile = kPmKeys * HD * 2;              // a K, V or Q tile
+  static constexpr int kSlots = HD == 128 ? 5 : 8;            // K and V tiles in the ring
+  static constexpr int kBytes = 1024 + (2 + kSlots) * kTile;
+};
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(kPmThreads) paged_prompt_kernel(const PromptParams p) {
-  constexpr int CPR = HD / 8;
-  constexpr int kTileBytes = kPmKeys * HD * 2;
-  extern __shared__ __align__(128) uint8_t smem[];   // 2 x (K tile, V tile)
-  __shared__ uint8_t lost[2][kPmKeys / 16];          // 16-key groups whose page id is outside the pool
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int kvh = blockIdx.y;
+__global__ void __launch_bounds__(kPmThreads, 1) paged_prompt_kernel(const __grid_constant__ PromptParams p) {
+  using S = PromptSmem<HD>;
+  constexpr int NS = S::kSlots, HALVES = HD / 64, HALF = kPmKeys * 128;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  __shared__ __align__(8) unsigned long long bar_q, bar_full[NS], bar_empty[NS], bar_s[2], bar_p[2], bar_o[2], bar_done;
+  __shared__ uint32_t tmem_s;
+  __shared__ volatile int abort_s, odd_s;
+  __shared__ volatile uint8_t lost_s[8];   // per key tile (mod 8): its 16-key groups whose page id is outside the pool
+
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int kvh = blockIdx.y, slice = blockIdx.z;
   pdl_wait();
   pdl_launch_dependents();
-  if (p.zero_tail) {
+  if (p.zero_tail && slice == 0) {
     for (int r = max(0, p.off[p.c.B]) + blockIdx.x; r < p.T; r += gridDim.x)
-      for (int i = tid; i < p.group * CPR; i += kPmThreads)
-        *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + r * p.o_t + (kvh * p.group + i / CPR) * p.o_h +
-                                  (i % CPR) * 8) = make_uint4(0, 0, 0, 0);
+      for (int i = tid; i < p.group * (HD / 8); i += kPmThreads)
+        *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + r * p.o_t + (kvh * p.group + i / (HD / 8)) * p.o_h +
+                                  (i % (HD / 8)) * 8) = make_uint4(0, 0, 0, 0);
   }
   int b, i0, n;
   if (!find_row_tile(p, gridDim.x - 1 - blockIdx.x, b, i0, n)) return;   // the longest rows first
   const int tok0 = p.off[b] + i0;
-  const int np = min(p.rp, n - i0);                  // positions of this tile
+  const int np = min(2 * p.rp, n - i0);              // positions of this CTA
+  const int ng = np > p.rp ? 2 : 1;                  // row tiles
   const int len = seq_len(p.c, b);
-  const int pos0 = p.c.lens[b] - n + i0;             // position of the first (negative: more rows than tokens)
-  const int last = min(pos0 + np, len) - 1;          // the last position any row has
-  const int lo0 = window_start(max(pos0, 0), p.window);
+  const int pos0 = p.c.lens[b] - n + i0;             // the first position (negative: more rows than tokens)
+  const int last = min(pos0 + np, len) - 1;          // the last one
   if (pos0 < 0 && tid == 0) lw_record_error(LW_ERR_BAD_INDEX);
-  const int hi_tile = last < 0 ? 0 : last / kPmKeys + 1;
-  const int ns = min((p.sinks + kPmKeys - 1) / kPmKeys, lo0 / kPmKeys);
+  const bool windowed = p.window > 0;
+  const int lo0 = window_start(max(pos0, 0), p.window);   // the first key the window of any row reaches
   const int w0 = lo0 / kPmKeys;
-  const int nt = p.window > 0 ? ns + max(0, hi_tile - w0) : hi_tile;
+  const int ns = windowed ? min((p.sinks + kPmKeys - 1) / kPmKeys, w0) : 0;   // tiles of first keys before it
+  const int nt_all = last < 0 ? 0 : ns + last / kPmKeys + 1 - w0;
+  const int t0 = (int)((long long)nt_all * slice / p.slices);
+  const int nt = (int)((long long)nt_all * (slice + 1) / p.slices) - t0;   // this slice's tiles
+  auto key_of = [&](int i) { return (t0 + i < ns ? t0 + i : w0 + t0 + i - ns) * kPmKeys; };
 
-  // rows of this lane: packed row r = (position r / group, head r % group)
-  int row[2], pos[2];
-  bool have[2];
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    row[e] = warp * 16 + g + 8 * e;
-    have[e] = row[e] < np * p.group;
-    pos[e] = have[e] ? min(pos0 + row[e] / p.group, len - 1) : -1;
-  }
-  uint32_t qa[HD / 16][4];
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const T* qp = static_cast<const T*>(p.q) + (long long)(tok0 + (have[e] ? row[e] / p.group : 0)) * p.q_t +
-                  (long long)(kvh * p.group + (have[e] ? row[e] % p.group : 0)) * p.q_h + 2 * t;
-#pragma unroll
-    for (int k = 0; k < HD / 16; ++k) {
-      qa[k][e] = have[e] ? *reinterpret_cast<const uint32_t*>(qp + k * 16) : 0u;
-      qa[k][2 + e] = have[e] ? *reinterpret_cast<const uint32_t*>(qp + k * 16 + 8) : 0u;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* base_ptr = smem_raw + (base - smem_u32(smem_raw));
+  auto slot_at = [&](int s) { return (uint32_t)(2 + s) * S::kTile; };
+
+  if (tid == 0) {
+    mbar_init(smem_u32(&bar_q), 1);
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(smem_u32(&bar_full[s]), 1);
+      mbar_init(smem_u32(&bar_empty[s]), 1);
     }
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(smem_u32(&bar_s[g]), 1);
+      mbar_init(smem_u32(&bar_p[g]), 4);
+      mbar_init(smem_u32(&bar_o[g]), 1);
+    }
+    mbar_init(smem_u32(&bar_done), 1);
+    abort_s = 0;
+    odd_s = 0;
+    fence_mbar_init();
   }
-  auto key_of = [&](int i) { return (p.window > 0 && i >= ns ? w0 + i - ns : i) * kPmKeys; };
-  auto tile_sees = [&](int key) { return key <= last && (p.window <= 0 || key >= lo0 || key < p.sinks); };
-  const uint32_t sm = smem_u32(smem);
-  auto load = [&](int i) {
-    if (i < nt) {
-      const int key0 = key_of(i);
-      const uint32_t dst = sm + (i & 1) * 2 * kTileBytes;
-      if (tid < kPmKeys / 16) {
-        bool bad = false;
-        const int first = key0 + tid * 16;   // the group's first key that some row sees
-        for (int k = first; k < first + 16; ++k)
-          if (tile_sees(k)) {
-            bad = page_id(p.c, b, k) < 0;
+  if (warp == kPmMmaWarp) {
+    tmem_alloc(smem_u32(&tmem_s), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_s;
+
+  // Bounded waits: the first to give up makes the others stop at their next one.
+  auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (abort_s) return false;
+    if (mbar_wait_bounded(bar, parity, kPmWaitNs)) return true;
+    abort_s = 1;
+    return false;
+  };
+  auto warp_wait = [&](uint32_t bar, uint32_t parity) -> bool {
+    return __shfl_sync(0xffffffffu, wait(bar, parity) ? 1u : 0u, 0) != 0;
+  };
+
+  if (warp == kPmTmaWarp) {
+    // ---- copies. Tile i's K is copy 2i of the ring, its V copy 2i + 1. Lane
+    // (page of the tile, half of the head dim) issues one box each.
+    const int pg = min(p.c.page_size, kPmKeys), npg = kPmKeys / pg;   // slots per box, boxes per tile and half
+    const int my_pg = lane % npg, my_half = lane / npg;
+    const bool mine = my_half < HALVES;
+    auto page_at = [&](int i) {   // page of this lane's part of tile i (no_page: zeros)
+      const int first = key_of(i) + my_pg * pg, end = first + pg - 1;
+      if (!(first <= last && (!windowed || end >= lo0 || first < p.sinks))) return p.no_page;
+      return page_id(p.c, b, first);
+    };
+    int issued = 0;
+    if (nt > 0) {
+      if (lane == 0) {
+        tma_prefetch_map(&p.tm_k);
+        tma_prefetch_map(&p.tm_v);
+        const uint32_t bytes = (uint32_t)(HALVES * 128 * p.group * p.rp);
+        mbar_arrive_expect_tx(smem_u32(&bar_q), bytes * ng);
+        for (int g = 0; g < ng; ++g)
+          for (int h = 0; h < HALVES; ++h)
+            tma_load_3d(base + g * S::kTile + h * HALF, &p.tm_q, h * 64, kvh * p.group, tok0 + g * p.rp,
+                        smem_u32(&bar_q));
+      }
+      int page = page_at(0);
+      bool ok = true;
+      for (int i = 0; i < nt && ok; ++i) {
+        const int key0 = key_of(i);
+        const int next = i + 1 < nt ? page_at(i + 1) : 0;   // asked for a tile ahead
+        // a page id outside the pool: its keys (16-key groups) are hidden, its copy is zeros
+        const uint32_t bad_boxes = __ballot_sync(0xffffffffu, page < 0) & ((1u << npg) - 1u);
+        if (lane == 0) {
+          uint32_t groups = 0;
+          for (int x = 0; x < npg; ++x)
+            if ((bad_boxes >> x) & 1u) groups |= ((1u << (pg / 16)) - 1u) << (x * (pg / 16));
+          lost_s[i & 7] = (uint8_t)groups;
+        }
+        const int w = page < 0 ? p.no_page : page;
+        const int slot = key0 & (p.c.page_size - 1);   // within a page of more than 128 slots
+        for (int kv = 0; kv < 2; ++kv) {
+          const int x = 2 * i + kv, s = x % NS;
+          if (x >= NS && !warp_wait(smem_u32(&bar_empty[s]), ((x / NS) - 1) & 1)) {
+            ok = false;
             break;
           }
-        lost[i & 1][tid] = bad;
-      }
-      for (int x = tid; x < kPmKeys * CPR; x += kPmThreads) {
-        const int r = x / CPR, c = x % CPR, key = key0 + r;
-        const int page = tile_sees(key) ? page_id(p.c, b, key) : -1;
-        const int slot = key & (p.c.page_size - 1);
-        const T *kp = static_cast<const T*>(p.q), *vp = kp;   // not read when there is no page
-        if (page >= 0) {
-          kp = static_cast<const T*>(p.c.k) + page * p.c.kp + kvh * p.c.kh + slot * p.c.ks + c * 8;
-          vp = static_cast<const T*>(p.c.v) + page * p.c.vp + kvh * p.c.vh + slot * p.c.vs + c * 8;
+          if (lane == 0) mbar_arrive_expect_tx(smem_u32(&bar_full[s]), S::kTile);
+          __syncwarp();
+          if (mine)
+            tma_load_4d(base + slot_at(s) + my_half * HALF + my_pg * pg * 128, kv ? &p.tm_v : &p.tm_k, my_half * 64, slot,
+                        kvh, w, smem_u32(&bar_full[s]));
+          __syncwarp();
+          issued = x + 1;
         }
-        const uint32_t at = dst + (uint32_t)(r * (HD * 2) + ((c ^ (r & 7)) << 4));
-        cp_async16(at, kp, page >= 0);
-        cp_async16(at + kTileBytes, vp, page >= 0);
+        page = next;
       }
+      // no copy may land after the CTA has ended (immediate unless a wait gave up)
+      if (lane == 0) {
+        mbar_wait_bounded(smem_u32(&bar_q), 0, kPmWaitNs);
+        for (int x = max(0, issued - NS); x < issued; ++x)
+          mbar_wait_bounded(smem_u32(&bar_full[x % NS]), (x / NS) & 1, kPmWaitNs);
+      }
+      __syncwarp();
     }
-    cp_async_commit();
-  };
-  float o[HD / 8][4];
+  } else if (warp == kPmMmaWarp) {
+    // ---- tensor cores
+    const bool leader = elect_one_sync();   // one thread issues everything: commits follow its instructions
+    constexpr uint32_t kFmt = std::is_same<T, __half>::value ? 0u : 1u;
+    constexpr uint32_t kCommon = (1u << 4) | (kFmt << 7) | (kFmt << 10) | ((uint32_t)(kPmRows >> 4) << 24);
+    constexpr uint32_t kDescS = kCommon | ((uint32_t)(kPmKeys >> 3) << 17);              // B = K, K-major
+    constexpr uint32_t kDescO = kCommon | ((uint32_t)(HD >> 3) << 17) | (1u << 16);      // B = V, N-major
+    auto scores = [&](int g, int s) {   // S_g = Q_g K^T
+      const uint64_t a = sw128_desc(base + g * S::kTile), k = sw128_desc(base + slot_at(s));
 #pragma unroll
-  for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-
-  load(0);
-  for (int i = 0; i < nt; ++i) {
-    load(i + 1);
-    cp_async_wait<1>();
-    __syncthreads();
-    const int key0 = key_of(i);
-    const uint32_t kt = sm + (i & 1) * 2 * kTileBytes, vt = kt + kTileBytes;
-    uint8_t* vptr = smem + (i & 1) * 2 * kTileBytes + kTileBytes;
-    // a tile that some row does not see whole
-    const bool partial = key0 + kPmKeys - 1 > pos0 || (p.window > 0 && key0 <= last - p.window);
-    bool odd = false;
-    if (partial) {
-      bool mine = false;
-      for (int x = tid; x < kPmKeys * CPR; x += kPmThreads) {
-        const uint4 v = lds128(vptr + x * 16);
-        mine |= has_nonfinite<T>(v.x) || has_nonfinite<T>(v.y) || has_nonfinite<T>(v.z) || has_nonfinite<T>(v.w);
+      for (int x = 0; x < HD / 16; ++x) {
+        const uint64_t o = (uint64_t)((x / 4) * (HALF >> 4) + (x % 4) * 2);
+        tc_mma_f16(tmem + g * kPmKeys, a + o, k + o, kDescS, x != 0);
       }
-      odd = __syncthreads_or(mine);
-    }
-    const uint8_t* gone = lost[i & 1];
-    auto sees = [&](int key, int e) {
-      return key <= pos[e] && !gone[(key - key0) >> 4] && (p.window <= 0 || pos[e] - key < p.window || key < p.sinks);
     };
-    if (odd) {
-      // each lane adds its rows' and columns' non-finite values, then they are cleared
+    auto values = [&](int g, int s, bool first) {   // O_g += P_g V
+      const uint64_t v = sw128_mn_desc(base + slot_at(s), HALF);
 #pragma unroll
-      for (int d8 = 0; d8 < HD / 8; ++d8) {
-        for (int r = 0; r < kPmKeys; ++r) {
-          const uint32_t u = *reinterpret_cast<const uint32_t*>(vptr + r * (HD * 2) + ((d8 ^ (r & 7)) << 4) + 4 * t);
-          if (!has_nonfinite<T>(u)) continue;
-          const float2 v = Elem<T>::unpack(u);
-          for (int e = 0; e < 2; ++e)
-            if (sees(key0 + r, e)) {
-              if (!isfinite(v.x)) o[d8][2 * e] += v.x;
-              if (!isfinite(v.y)) o[d8][2 * e + 1] += v.y;
+      for (int x = 0; x < kPmKeys / 16; ++x)
+        tc_mma_f16_ts(tmem + 2 * kPmKeys + g * HD, tmem + g * kPmKeys + 8 * x, v + (uint64_t)(x * (2048 >> 4)), kDescO,
+                      !first || x != 0);
+    };
+    if (nt > 0) {
+      bool ok = warp_wait(smem_u32(&bar_q), 0) && warp_wait(smem_u32(&bar_full[0]), 0);
+      if (ok) {
+        tc_fence_after();
+        if (leader) {
+          for (int g = 0; g < ng; ++g) {
+            scores(g, 0);
+            tc_commit(smem_u32(&bar_s[g]));
+          }
+          tc_commit(smem_u32(&bar_empty[0]));
+        }
+        __syncwarp();
+      }
+      for (int i = 0; i < nt && ok; ++i) {
+        const int xv = 2 * i + 1, sv = xv % NS, xk = 2 * i + 2, sk = xk % NS;
+        ok = warp_wait(smem_u32(&bar_full[sv]), (xv / NS) & 1);
+        for (int g = 0; g < ng && ok; ++g) {
+          ok = warp_wait(smem_u32(&bar_p[g]), i & 1);
+          if (ok && g == 0 && i + 1 < nt) ok = warp_wait(smem_u32(&bar_full[sk]), (xk / NS) & 1);
+          if (!ok) break;
+          tc_fence_after();
+          if (leader) {
+            values(g, sv, i == 0);
+            if (g == ng - 1) tc_commit(smem_u32(&bar_empty[sv]));
+            if (i + 1 < nt) {
+              scores(g, sk);
+              tc_commit(smem_u32(&bar_s[g]));
+              if (g == ng - 1) tc_commit(smem_u32(&bar_empty[sk]));
+            } else {
+              tc_commit(smem_u32(&bar_o[g]));
             }
+          }
+          __syncwarp();
         }
       }
-      __syncthreads();
-      for (int x = tid; x < kPmKeys * CPR * 8; x += kPmThreads) {
-        uint16_t* h = reinterpret_cast<uint16_t*>(vptr) + x;
-        if ((*h & Elem<T>::kExpMask) == Elem<T>::kExpMask) *h = 0;
+      // tensor memory may not be released under a running instruction
+      if (leader) {
+        tc_commit(smem_u32(&bar_done));
+        mbar_wait_bounded(smem_u32(&bar_done), 0, kPmWaitNs);
       }
-      __syncthreads();
+      __syncwarp();
     }
-    float sc[kPmKeys / 8][4];
+  } else if (warp / 4 < ng) {
+    // ---- softmax of row tile g, row r
+    const int g = warp >> 2, r = tid & 127;
+    const int npos = min(p.rp, np - g * p.rp);
+    const bool have = r < npos * p.group;
+    const int first_pos = pos0 + g * p.rp, last_pos = min(first_pos + npos, len) - 1;
+    const int pos = have ? min(first_pos + r / p.group, len - 1) : -1;
+    const int lo = windowed ? pos - p.window : -1;   // keys above lo, or below sinks
+    const int sinks = windowed ? p.sinks : 0;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + lanes + g * kPmKeys, to = tmem + lanes + 2 * kPmKeys + g * HD;
+    auto sees = [&](int key) { return key <= pos && (key > lo || key < sinks); };
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int i = 0; i < nt; ++i) {
+      if (!(ok = warp_wait(smem_u32(&bar_s[g]), i & 1))) break;
+      tc_fence_after();
+      const int key0 = key_of(i);
+      uint32_t s[4][32];
 #pragma unroll
-    for (int x = 0; x < kPmKeys / 8; ++x) sc[x][0] = sc[x][1] = sc[x][2] = sc[x][3] = 0.f;
-    {
-      const int r8 = (lane >> 4) * 8 + (lane & 7), cb = (lane >> 3) & 1;
+      for (int x = 0; x < 4; ++x) tmem_ld32(ts + 32 * x, s[x]);
+      tmem_wait_ld();
 #pragma unroll
-      for (int k = 0; k < HD / 16; ++k)
+      for (int x = 0; x < 4; ++x) tmem_regs_ready(s[x]);
+      const uint32_t lost = lost_s[i & 7];
+      const bool partial = key0 + kPmKeys - 1 > first_pos || (windowed && key0 <= last_pos - p.window) || lost;
+      if (partial) {
 #pragma unroll
-        for (int x = 0; x < kPmKeys / 16; ++x) {
-          const int r = x * 16 + r8;
-          uint32_t f[4];
-          ldmatrix_x4(kt + (uint32_t)(r * (HD * 2) + (((2 * k + cb) ^ (r & 7)) << 4)), f);
-          mma_16816<T>(sc[2 * x], qa[k][0], qa[k][1], qa[k][2], qa[k][3], f[0], f[1]);
-          mma_16816<T>(sc[2 * x + 1], qa[k][0], qa[k][1], qa[k][2], qa[k][3], f[2], f[3]);
-        }
-    }
-    float mx[2] = {-INFINITY, -INFINITY};
+        for (int x = 0; x < 4; ++x)
 #pragma unroll
-    for (int x = 0; x < kPmKeys / 8; ++x)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        sc[x][e] = sees(key0 + x * 8 + 2 * t + (e & 1), e >> 1) ? sc[x][e] * p.scale_log2 : -INFINITY;
-        mx[e >> 1] = fmaxf(mx[e >> 1], sc[x][e]);
+          for (int e = 0; e < 32; ++e)
+            if (!sees(key0 + 32 * x + e) || ((lost >> (2 * x + e / 16)) & 1u)) s[x][e] = __float_as_uint(-INFINITY);
       }
-    float corr[2], base[2];
+      float mx[4];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
-      mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
-      const float mn = fmaxf(m[e], mx[e]);
-      corr[e] = m[e] == -INFINITY ? 1.f : exp2f(m[e] - mn);
-      base[e] = mn == -INFINITY ? 0.f : mn;
-      m[e] = mn;
-      l[e] *= corr[e];
-    }
+      for (int x = 0; x < 4; ++x) {
+        mx[x] = __uint_as_float(s[x][0]);
 #pragma unroll
-    for (int x = 0; x < kPmKeys / 8; ++x)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        sc[x][e] = exp2f(sc[x][e] - base[e >> 1]);
-        l[e >> 1] += sc[x][e];
+        for (int e = 1; e < 32; ++e) mx[x] = fmaxf(mx[x], __uint_as_float(s[x][e]));
       }
+      const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+      if (i == 0) {
+        m = mt;
+      } else {
+        const bool grow = mt > m + kPmGrow;
+        if (__any_sync(0xffffffffu, grow)) {
+          // O's update i - 1 is complete (S(i) was issued after it)
+          const float f = !grow ? 1.f : (m == -INFINITY ? 0.f : ex2(m - mt));
+          if (grow) m = mt;
+          l *= f;
 #pragma unroll
-    for (int x = 0; x < HD / 8; ++x) {
-      o[x][0] *= corr[0];
-      o[x][1] *= corr[0];
-      o[x][2] *= corr[1];
-      o[x][3] *= corr[1];
-    }
-    {
-      const int r8 = ((lane >> 3) & 1) * 8 + (lane & 7), cb = lane >> 4;
+          for (int x = 0; x < HD / 32; ++x) {
+            uint32_t o[32];
+            tmem_ld32(to + 32 * x, o);
+            tmem_wait_ld();
+            tmem_regs_ready(o);
 #pragma unroll
-      for (int x = 0; x < kPmKeys / 16; ++x) {
-        const uint32_t a0 = Elem<T>::pack(sc[2 * x][0], sc[2 * x][1]), a1 = Elem<T>::pack(sc[2 * x][2], sc[2 * x][3]);
-        const uint32_t a2 = Elem<T>::pack(sc[2 * x + 1][0], sc[2 * x + 1][1]);
-        const uint32_t a3 = Elem<T>::pack(sc[2 * x + 1][2], sc[2 * x + 1][3]);
-        const int r = x * 16 + r8;
-#pragma unroll
-        for (int d = 0; d < HD / 16; ++d) {
-          uint32_t f[4];
-          ldmatrix_x4_t(vt + (uint32_t)(r * (HD * 2) + (((2 * d + cb) ^ (r & 7)) << 4)), f);
-          mma_16816<T>(o[2 * d], a0, a1, a2, a3, f[0], f[1]);
-          mma_16816<T>(o[2 * d + 1], a0, a1, a2, a3, f[2], f[3]);
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            tmem_st32(to + 32 * x, o);
+          }
         }
       }
+      const float sub = m == -INFINITY ? 0.f : m;   // no key seen yet: every weight is 0
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        // weights rounded to T for the second product: half a step each, averaged
+        // over the keys; their sum is that of the unrounded ones
+        uint32_t w[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const int x = 2 * h + e / 16, y = (2 * e) % 32;
+          const float a = ex2(fmaf(__uint_as_float(s[x][y]), p.scale_log2, -sub));
+          const float c = ex2(fmaf(__uint_as_float(s[x][y + 1]), p.scale_log2, -sub));
+          sum[e & 1] += a;
+          sum[2 + (e & 1)] += c;
+          w[e] = Elem<T>::pack(a, c);
+        }
+        tmem_st32(ts + 32 * h, w);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      if (g == 0 && (key0 + kPmKeys - 1 > pos0 || (windowed && key0 <= last - p.window))) {
+        // V's row r of a tile that some row does not see whole
+        const int xv = 2 * i + 1;
+        if (!(ok = warp_wait(smem_u32(&bar_full[xv % NS]), (xv / NS) & 1))) break;
+        uint8_t* row = base_ptr + slot_at(xv % NS) + r * 128;
+        const int key = key0 + r;
+        const bool anyone = key <= last && (!windowed || key >= lo0 || key < p.sinks);
+        for (int c = 0; c < HALVES * 8; ++c) {
+          uint8_t* at = row + (c / 8) * HALF + (((c + r) & 7) << 4);   // the order does not matter: spread over the banks
+          const uint4 v = lds128(at);
+          uint32_t u[4] = {v.x, v.y, v.z, v.w};
+          bool hit = false;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) hit |= has_nonfinite<T>(u[e]);
+          if (hit) {
+            constexpr uint32_t kLo = Elem<T>::kExpMask, kHi = kLo << 16;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if ((u[e] & kLo) == kLo) u[e] &= 0xFFFF0000u;
+              if ((u[e] & kHi) == kHi) u[e] &= 0x0000FFFFu;
+            }
+            sts128(at, make_uint4(u[0], u[1], u[2], u[3]));
+            if (anyone) odd_s = 1;
+          }
+        }
+        fence_proxy_async_smem();   // before the tensor cores read it
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&bar_p[g]));
     }
-    __syncthreads();   // the stage is free for tile i + 2
+    // ---- the row's result
+    if (nt > 0 && ok) {
+      ok = warp_wait(smem_u32(&bar_o[g]), 0);
+      tc_fence_after();
+    }
+    if (ok) {
+      const int tok = tok0 + g * p.rp + (have ? r / p.group : 0), head = kvh * p.group + (have ? r % p.group : 0);
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const bool odd = odd_s;
+      const long long at = ((long long)slice * p.T + tok) * p.nq + head;
+      if (p.slices > 1 && have) p.part_ml[at] = make_float2(nt > 0 ? m : -INFINITY, l);
+#pragma unroll 1
+      for (int x = 0; x < HD / 32; ++x) {
+        uint32_t o[32];
+        if (nt > 0) {
+          tmem_ld32(to + 32 * x, o);
+          tmem_wait_ld();
+          tmem_regs_ready(o);
+        } else {
+          if (p.slices > 1) break;   // nothing of this slice is read
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0u;
+        }
+        if (odd && have) {
+          // the values that were cleared and that this row sees
+          for (int i = 0; i < nt; ++i) {
+            const int key0 = key_of(i);
+            if (!(key0 + kPmKeys - 1 > pos0 || (windowed && key0 <= last - p.window))) continue;
+            for (int key = key0; key < key0 + kPmKeys; ++key) {
+              if (!sees(key)) continue;
+              const int page = page_id(p.c, b, key);
+              if (page < 0) continue;
+              const T* v = static_cast<const T*>(p.c.v) + page * p.c.vp + kvh * p.c.vh +
+                           (key & (p.c.page_size - 1)) * p.c.vs + 32 * x;
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                const float f = static_cast<float>(v[e]);
+                if (!isfinite(f)) o[e] = __float_as_uint(__uint_as_float(o[e]) + f);
+              }
+            }
+          }
+        }
+        if (!have) continue;
+        if (p.slices > 1) {
+          float4* dst = reinterpret_cast<float4*>(p.part_o + at * HD + 32 * x);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            dst[e] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]),
+                                 __uint_as_float(o[4 * e + 3]));
+        } else {
+          uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + tok * p.o_t + head * p.o_h + 32 * x);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t u[4];
+#pragma unroll
+            for (int f = 0; f < 4; ++f)
+              u[f] = Elem<T>::pack(__uint_as_float(o[8 * e + 2 * f]) * inv, __uint_as_float(o[8 * e + 2 * f + 1]) * inv);
+            dst[e] = make_uint4(u[0], u[1], u[2], u[3]);
+          }
+        }
+      }
+    }
   }
-  cp_async_wait<0>();
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
-    l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
-    if (!have[e]) continue;
-    const float inv = l[e] == 0.f ? 0.f : 1.f / l[e];
-    T* dst = static_cast<T*>(p.out) + (long long)(tok0 + row[e] / p.group) * p.o_t +
-             (long long)(kvh * p.group + row[e] % p.group) * p.o_h + 2 * t;
-#pragma unroll
-    for (int x = 0; x < HD / 8; ++x)
-      *reinterpret_cast<uint32_t*>(dst + x * 8) = Elem<T>::pack(o[x][2 * e] * inv, o[x][2 * e + 1] * inv);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kPmMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
   }
+}
+
+// Joins the key slices of every row, in order. A row per HD / 4 threads.
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) paged_prompt_join_kernel(const __grid_constant__ PromptParams p) {
+  pdl_wait();
+  pdl_launch_dependents();
+  constexpr int TPR = HD / 4;
+  const long long row = (long long)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+  if (row >= (long long)p.T * p.nq) return;
+  const int tok = (int)(row / p.nq), head = (int)(row - (long long)tok * p.nq), d = (threadIdx.x % TPR) * 4;
+  if (row_sequence(p.off, p.c.B, tok) < 0) return;   // behind the last sequence: not ours
+  const long long step = (long long)p.T * p.nq;
+  float M = -INFINITY;
+  for (int i = 0; i < p.slices; ++i) M = fmaxf(M, p.part_ml[i * step + row].x);
+  float L = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < p.slices; ++i) {
+    const float2 ml = p.part_ml[i * step + row];
+    if (ml.x == -INFINITY) continue;   // a slice without a key for this row
+    const float f = ex2(ml.x - M);
+    const float4 o = *reinterpret_cast<const float4*>(p.part_o + (i * step + row) * HD + d);
+    L = fmaf(ml.y, f, L);
+    acc.x = fmaf(o.x, f, acc.x);
+    acc.y = fmaf(o.y, f, acc.y);
+    acc.z = fmaf(o.z, f, acc.z);
+    acc.w = fmaf(o.w, f, acc.w);
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  uint2 u = make_uint2(Elem<T>::pack(acc.x * inv, acc.y * inv), Elem<T>::pack(acc.z * inv, acc.w * inv));
+  *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + tok * p.o_t + head * p.o_h + d) = u;
 }
 
 }  // namespace lw
@@ -276,8 +533,9 @@ int check(const lw_paged_attention_args* a) {
   int st = lw_host::check_cache(a->cache);
   if (st) return st;
   if (a->tokens < 0 || a->n_q_heads <= 0 || a->n_q_heads % a->cache.n_kv_heads || a->sinks < 0) return LW_ERR_BAD_SHAPE;
+  if (!(a->scale > 0.f) || a->scale > 3.0e38f) return LW_ERR_BAD_SHAPE;   // the maximum is taken before scaling
   if (!a->q_offsets && a->tokens != a->cache.batch) return LW_ERR_BAD_SHAPE;
-  if (a->q_offsets && a->n_q_heads / a->cache.n_kv_heads > lw::kPmRows) return LW_ERR_UNSUPPORTED;
+  if (a->q_offsets && a->n_q_heads / a->cache.n_kv_heads > 64) return LW_ERR_UNSUPPORTED;
   if (a->tokens == 0) return LW_OK;
   if (a->cache.batch == 0) return LW_ERR_BAD_SHAPE;
   if (!a->q || !a->out) return LW_ERR_NULL_POINTER;
@@ -287,14 +545,51 @@ int check(const lw_paged_attention_args* a) {
   return LW_OK;
 }
 
+struct PromptPlan {
+  int group, rp, slices;
+  size_t o_off, bytes;
+};
+
+PromptPlan prompt_plan(const lw_paged_attention_args* a) {
+  PromptPlan d;
+  d.group = a->n_q_heads / a->cache.n_kv_heads;
+  d.rp = lw::kPmRows / d.group;
+  // Keys are cut into slices only where the row tiles leave SMs idle, as many
+  // slices as fill them, none below four key tiles.
+  const long long R = 2 * d.rp;
+  const long long ctas = ((long long)a->tokens + a->cache.batch * (R - 1)) / R * a->cache.n_kv_heads;
+  long long keys = (long long)a->cache.table_width * a->cache.page_size;
+  if (a->window > 0) keys = std::min(keys, (long long)a->window + a->sinks + R);
+  const long long most = std::min(keys / (4 * lw::kPmKeys), lw_host::sm_count() / std::max(1ll, ctas));
+  d.slices = (int)std::max(1ll, std::min(most, 64ll));
+  const size_t rows = (size_t)a->tokens * a->n_q_heads * d.slices;
+  d.o_off = (rows * sizeof(float2) + 255) & ~(size_t)255;
+  d.bytes = d.slices > 1 ? d.o_off + rows * a->cache.head_dim * sizeof(float) : 0;
+  return d;
+}
+
 template <typename T, int HD>
 cudaError_t prompt_launch(const lw::PromptParams& p, cudaStream_t s, bool pdl) {
-  constexpr int smem = 4 * lw::kPmKeys * HD * 2;
+  constexpr int smem = lw::PromptSmem<HD>::kBytes;
   auto kern = lw::paged_prompt_kernel<T, HD>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  return lw_launch(kern, dim3((unsigned)(p.T / p.rp + p.c.B), (unsigned)p.c.nkv), dim3(lw::kPmThreads), smem, s, pdl,
+  e = lw_launch(kern, dim3((unsigned)(p.T / (2 * p.rp) + p.c.B), (unsigned)p.c.nkv, (unsigned)p.slices),
+                dim3(lw::kPmThreads), smem, s, pdl, p);
+  if (e != cudaSuccess || p.slices == 1) return e;
+  const long long rows = (long long)p.T * p.nq, per = 256 / (HD / 4);
+  if ((rows + per - 1) / per > 0x7FFFFFFFll) return cudaErrorInvalidValue;
+  return lw_launch(lw::paged_prompt_join_kernel<T, HD>, dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, s, true,
                    p);
+}
+
+// Tensor map of a pool [pages][heads][slots][head_dim] by its strides.
+bool pool_map(CUtensorMap* m, CUtensorMapDataType type, const void* base, const lw_paged_cache& c, const long long* st) {
+  const uint64_t dims[4] = {(uint64_t)c.head_dim, (uint64_t)c.page_size, (uint64_t)c.n_kv_heads,
+                            (uint64_t)std::max(1, c.n_pages)};
+  const uint64_t strides[3] = {(uint64_t)st[2] * 2, (uint64_t)st[1] * 2, (uint64_t)st[0] * 2};
+  const uint32_t box[4] = {64, (uint32_t)std::min(c.page_size, lw::kPmKeys), 1, 1};
+  return lw::encode_nd_sw128(m, type, base, 4, dims, strides, box);
 }
 
 }  // namespace
@@ -305,7 +600,7 @@ extern "C" {
 
 size_t lw_paged_attention_workspace_size(const lw_paged_attention_args* a) {
   if (check(a) != LW_OK || a->tokens == 0) return 0;
-  return a->q_offsets ? 0 : lw_paged_decode_workspace(a);
+  return a->q_offsets ? prompt_plan(a).bytes : lw_paged_decode_workspace(a);
 }
 
 int lw_paged_attention(const lw_paged_attention_args* a, lw_stream_t stream) {
@@ -318,23 +613,37 @@ int lw_paged_attention(const lw_paged_attention_args* a, lw_stream_t stream) {
   cudaGetLastError();
   if (!a->q_offsets) return lw_paged_decode(a, s);
   if (a->cache.n_kv_heads > 65535) return LW_ERR_UNSUPPORTED;
+  const PromptPlan d = prompt_plan(a);
   lw::PromptParams p = {};
   p.c = lw_host::view_of(a->cache);
-  p.q = a->q;
   p.out = a->out;
-  p.q_t = a->q_strides[0];
-  p.q_h = a->q_strides[1];
   p.o_t = a->out_strides[0];
   p.o_h = a->out_strides[1];
   p.T = a->tokens;
   p.nq = a->n_q_heads;
-  p.group = a->n_q_heads / a->cache.n_kv_heads;
-  p.rp = lw::kPmRows / p.group;
+  p.group = d.group;
+  p.rp = d.rp;
+  p.no_page = std::max(1, a->cache.n_pages);
   p.off = a->q_offsets;
   p.window = a->window;
   p.sinks = a->sinks;
   p.scale_log2 = a->scale * 1.4426950408889634f;
   p.zero_tail = a->zero_tail;
+  p.slices = d.slices;
+  p.part_ml = static_cast<float2*>(a->workspace);
+  p.part_o = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + d.o_off);
+  const CUtensorMapDataType type =
+      a->cache.dtype == LW_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const uint64_t dims[3] = {(uint64_t)a->cache.head_dim, (uint64_t)a->n_q_heads, (uint64_t)a->tokens};
+  const uint64_t strides[2] = {(uint64_t)a->q_strides[1] * 2, (uint64_t)a->q_strides[0] * 2};
+  const uint32_t box[3] = {64, (uint32_t)d.group, (uint32_t)d.rp};
+  // an empty pool has no address: every copy is past its end then
+  const void* kb = a->cache.n_pages ? a->cache.k_pages : a->q;
+  const void* vb = a->cache.n_pages ? a->cache.v_pages : a->q;
+  if (!lw::encode_nd_sw128(&p.tm_q, type, a->q, 3, dims, strides, box) ||
+      !pool_map(&p.tm_k, type, kb, a->cache, a->cache.k_strides) ||
+      !pool_map(&p.tm_v, type, vb, a->cache, a->cache.v_strides))
+    return LW_ERR_UNSUPPORTED;   // strides that a tensor map does not take
   const bool pdl = a->pdl != 0;
   cudaError_t e;
   if (a->cache.dtype == LW_DTYPE_F16)

@@ -58,4 +58,24 @@ inline bool encode_3d(CUtensorMap* m, CUtensorMapDataType type, const void* ptr,
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// N-D tiled tensor map of 16-bit elements with 128-byte swizzle: dims[0] is
+// contiguous, strides (bytes) are those of dims 1 .. n - 1; a dimension of one
+// element takes any stride.
+inline bool encode_nd_sw128(CUtensorMap* m, CUtensorMapDataType type, const void* ptr, int n, const uint64_t* dims,
+                            const uint64_t* strides, const uint32_t* box) {
+  auto enc = tensor_map_encoder();
+  if (!enc || n < 2 || n > 5) return false;
+  cuuint64_t d[5], st[4];
+  cuuint32_t b[5], elem[5];
+  for (int i = 0; i < n; ++i) {
+    d[i] = dims[i];
+    b[i] = box[i];
+    elem[i] = 1;
+    if (i) st[i - 1] = dims[i] == 1 ? 16 : strides[i - 1];
+  }
+  return enc(m, type, n, const_cast<void*>(ptr), d, st, b, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 }  // namespace lw

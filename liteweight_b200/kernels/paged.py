@@ -217,7 +217,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
     Args:
         q:      [batch, q heads, head_dim], in the cache's dtype
-        scale:  of the scores, head_dim ** -0.5 by default
+        scale:  of the scores, above 0; head_dim ** -0.5 by default
         out:    [batch, q heads, head_dim] (may not overlap q)
     """
     return _attention(q, k_pages, v_pages, page_table, kv_lens, None, window, sinks, scale, out)

@@ -61,7 +61,8 @@ def test_bad_caches_are_refused(lib, kw, status):
 
 @pytest.mark.parametrize("kw,status", [
     (dict(q=None), 1), (dict(out=None), 1), (dict(tokens=3), 2), (dict(n_q_heads=6), 2), (dict(n_q_heads=0), 2),
-    (dict(sinks=-1), 2), (dict(q=FAKE + 8), 4), (dict(out_strides=(1024, 130)), 4), (dict(tokens=-1), 2),
+    (dict(sinks=-1), 2), (dict(scale=0.0), 2), (dict(scale=-1.0), 2), (dict(scale=float("nan")), 2),
+    (dict(scale=float("inf")), 2), (dict(q=FAKE + 8), 4), (dict(out_strides=(1024, 130)), 4), (dict(tokens=-1), 2),
     (dict(workspace=None), 7), (dict(workspace=FAKE, workspace_bytes=256), 7),
     (dict(workspace=FAKE + 16, workspace_bytes=1 << 30), 4),
     (dict(q_offsets=FAKE + 2), 4), (dict(q_offsets=FAKE, n_q_heads=4 * 65), 5),
