@@ -81,6 +81,13 @@ LW_DEV void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+// 2^x (a result below the normal range is 0).
+LW_DEV float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // ------------------------------------------------------------- the cache
 
 struct PagedView {
@@ -113,8 +120,7 @@ LW_DEV int page_id(const PagedView& c, int b, int tok) {
   return -1;
 }
 
-// First position whose window reaches back to key `lo` is not needed here: this
-// is the first key that position p sees through its window.
+// The first key that position p sees through its window.
 LW_DEV int window_start(int p, int window) { return window > 0 ? max(0, p - window + 1) : 0; }
 
 // Sequence of row t: the b with off[b] <= t < off[b + 1], or -1.

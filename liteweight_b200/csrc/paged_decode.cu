@@ -6,20 +6,29 @@
 //
 // Bound by reading the visible keys and values once. The work is cut into
 // tiles of 16 consecutive token positions (one page each: a page is a multiple
-// of 16 slots) of one item = (sequence, kv head, block of up to 16 query heads
-// of its group). All items' tiles form one line, and every CTA of a grid of one
-// per SM takes an equal run of it, so sequences of any lengths keep all SMs
-// equally busy; a run's eight warps take its tiles in turn. A warp streams its
-// tiles through a private ring of shared-memory stages (cp.async, no CTA
-// barrier), computes S = Q K^T and O += P V with mma.sync (the query heads of
-// the group are the MMA's rows, so K and V are read once for all of them) and
-// keeps an online softmax in fp32. At the end of an item the warps merge in
-// shared memory; an item that lies in one run is written at once, otherwise each
-// run leaves (max, sum, fp32 accumulator) in the workspace and a second kernel
-// joins them in order: the same bits on every call.
+// of 16 slots) of one item = (sequence, kv head, block of up to ROWS query
+// heads of its group). A warp streams tiles through a private ring of
+// shared-memory stages (cp.async, no CTA barrier), computes S = Q K^T and
+// O += P V with mma.sync (the query heads are the MMA's rows, so K and V are
+// read once for all of them) and keeps an online softmax in fp32.
+//
+// Long or many sequences: all items' tiles form one line, and every warp of a
+// grid of one CTA per SM takes an equal run of it, so sequences of any lengths
+// keep all SMs equally busy. An item that lies in one run is written by its
+// warp. Other pieces wait in shared memory until the CTA's warps are done; those
+// of one item are merged there, and what continues in another CTA is left as
+// (max, sum, fp32 accumulator) in the workspace, which a second kernel joins in
+// order: the same bits on every call.
+//
+// Few short sequences: a cluster of up to eight CTAs takes an item and merges
+// through distributed shared memory: one launch, no workspace.
 //
 // Hidden keys of a tile are zero-filled by the copy, so what their slots hold
 // (NaN included) never meets the tensor cores.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
 #include "paged.cuh"
 
 namespace lw {
@@ -27,26 +36,24 @@ namespace lw {
 constexpr int kPdWarps = 8;
 constexpr int kPdThreads = kPdWarps * 32;
 constexpr int kPdTile = 16;      // keys per tile
-constexpr int kPdRows = 16;      // query heads per item (MMA rows)
-constexpr int kPdMinRun = 8;     // tiles a CTA takes at least: one per warp
 
 struct PagedDecodeParams {
   PagedView c;
   const void* q;
   void* out;
   long long q_b, q_h, o_b, o_h;
-  int nq, group, hblocks;   // group = nq / nkv; hblocks = blocks of kPdRows heads in it
+  int group, hblocks;       // group = query heads per kv head; hblocks = blocks of ROWS heads in it
   int window, sinks;
   float scale_log2;
-  int grid;                 // CTAs of the first kernel
-  int2* meta;               // [items]: first run << 1 | starts inside it, runs (0: nothing to join)
-  float* part;              // [2 * grid][kPdRows][HD + 2]
+  int2* meta;               // [items]: first CTA, CTAs that hold a piece (0: nothing to join)
+  float* part;              // [2 * grid][ROWS][HD + 8]
 };
 
 // The tiles a sequence's newest position sees: [0, ns) and [w0, w0 + nt - ns).
 struct TileSpan {
   int len, lo, sinks;   // keys [lo, len) and [0, sinks) are visible
   int ns, w0, nt;
+  LW_DEV int key0(int tile) const { return (tile < ns ? tile : w0 + tile - ns) * kPdTile; }
 };
 
 LW_DEV TileSpan tile_span(const PagedDecodeParams& p, int len) {
@@ -60,33 +67,208 @@ LW_DEV TileSpan tile_span(const PagedDecodeParams& p, int len) {
   return s;
 }
 
-// A place on the line of tiles: sequence b, its span, item within it.
+// Sizes of a kernel's shared memory: a ring per warp, then pieces [warps][ROWS][HD + 8]
+// (accumulator, maximum, sum; the stride keeps the fragment stores off each other's banks).
+template <int HD, int ROWS>
+struct DecodeShape {
+  static constexpr int kTileBytes = kPdTile * HD * 2;           // K or V of a tile
+  static constexpr int kRing = ROWS == 8 ? 24576 : 16384;       // per warp
+  static constexpr int kStages = kRing / (2 * kTileBytes);
+  static constexpr int kStride = HD + 8;
+  static constexpr int kPiece = ROWS * kStride;                 // floats
+  static constexpr int kBytes = kPdWarps * (kRing + kPiece * 4);
+};
+
+// One warp's share of an item: queries as MMA fragments, the online softmax of
+// rows g and g + 8 (g + 8 with ROWS = 16 only), the accumulator.
+template <typename T, int HD, int ROWS>
+struct WarpItem {
+  using S = DecodeShape<HD, ROWS>;
+  static constexpr int R = ROWS / 8;
+  uint32_t qa[HD / 16][2 * R];
+  float o[HD / 8][4];
+  float m[R], l[R];
+
+  LW_DEV static void load_q(const PagedDecodeParams& p, int b, int head0, int rows, int lane,
+                            uint32_t (&f)[HD / 16][2 * R]) {
+    const int g = lane >> 2, t = lane & 3;
+    const T* qp = static_cast<const T*>(p.q) + b * p.q_b + (long long)head0 * p.q_h + 2 * t;
+#pragma unroll
+    for (int k = 0; k < HD / 16; ++k)
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const bool ok = g + 8 * r < rows;
+        const T* at = qp + (g + 8 * r) * p.q_h + k * 16;
+        f[k][r] = ok ? *reinterpret_cast<const uint32_t*>(at) : 0u;
+        f[k][R + r] = ok ? *reinterpret_cast<const uint32_t*>(at + 8) : 0u;
+      }
+  }
+
+  LW_DEV void clear() {
+#pragma unroll
+    for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) m[r] = -INFINITY, l[r] = 0.f;
+  }
+
+  // Keys key0 .. key0 + 15 of the stage at `kt` (K tile, then V tile; 16-byte
+  // chunk c of row r at chunk c ^ (r & 7)).
+  LW_DEV void tile(const PagedDecodeParams& p, const TileSpan& sp, int key0, bool kept, uint32_t kt, int lane) {
+    const int t = lane & 3;
+    float sc[2][4] = {};
+    {
+      // matrices of 8 keys x 8 dims: (keys 0-7 | 8-15) x (dims 0-7 | 8-15) of a k-step
+      const int r = (lane >> 4) * 8 + (lane & 7), cb = (lane >> 3) & 1;
+#pragma unroll
+      for (int k = 0; k < HD / 16; ++k) {
+        uint32_t b[4];
+        ldmatrix_x4(kt + (uint32_t)(r * (HD * 2) + (((2 * k + cb) ^ (r & 7)) << 4)), b);
+        const uint32_t a1 = R == 2 ? qa[k][R - 1] : 0u, a3 = R == 2 ? qa[k][2 * R - 1] : 0u;
+        mma_16816<T>(sc[0], qa[k][0], a1, qa[k][R], a3, b[0], b[1]);
+        mma_16816<T>(sc[1], qa[k][0], a1, qa[k][R], a3, b[2], b[3]);
+      }
+    }
+    const bool whole = kept && key0 + kPdTile <= sp.len && (key0 >= sp.lo || key0 + kPdTile <= sp.sinks);
+    if (!whole) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int key = key0 + n * 8 + 2 * t + (e & 1);
+          if (!(kept && key < sp.len && (key >= sp.lo || key < sp.sinks))) sc[n][e] = -INFINITY;
+        }
+    }
+    float corr[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float mx = fmaxf(fmaxf(sc[0][2 * r], sc[0][2 * r + 1]), fmaxf(sc[1][2 * r], sc[1][2 * r + 1]));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const float mn = fmaxf(m[r], mx * p.scale_log2);
+      const float base = mn == -INFINITY ? 0.f : mn;   // no key seen yet: every weight is 0
+      corr[r] = ex2(m[r] - base);
+      m[r] = mn;
+      float sum = 0.f;
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 2 * r; e < 2 * r + 2; ++e) {
+          sc[n][e] = ex2(fmaf(sc[n][e], p.scale_log2, -base));
+          sum += sc[n][e];
+        }
+      l[r] = fmaf(l[r], corr[r], sum);
+    }
+    // the weights lie in [0, 1]: rounded to T for the second product, half a
+    // step each, averaged over the keys; their sum stays in fp32
+    const uint32_t a0 = Elem<T>::pack(sc[0][0], sc[0][1]), a2 = Elem<T>::pack(sc[1][0], sc[1][1]);
+    const uint32_t a1 = R == 2 ? Elem<T>::pack(sc[0][2], sc[0][3]) : 0u;
+    const uint32_t a3 = R == 2 ? Elem<T>::pack(sc[1][2], sc[1][3]) : 0u;
+#pragma unroll
+    for (int i = 0; i < HD / 8; ++i) {
+      o[i][0] *= corr[0];
+      o[i][1] *= corr[0];
+      if constexpr (R == 2) {
+        o[i][2] *= corr[R - 1];
+        o[i][3] *= corr[R - 1];
+      }
+    }
+    const uint32_t vt = kt + S::kTileBytes;
+    const int r = ((lane >> 3) & 1) * 8 + (lane & 7), cb = lane >> 4;
+#pragma unroll
+    for (int d = 0; d < HD / 16; ++d) {
+      uint32_t b[4];
+      ldmatrix_x4_t(vt + (uint32_t)(r * (HD * 2) + (((2 * d + cb) ^ (r & 7)) << 4)), b);
+      mma_16816<T>(o[2 * d], a0, a1, a2, a3, b[0], b[1]);
+      mma_16816<T>(o[2 * d + 1], a0, a1, a2, a3, b[2], b[3]);
+    }
+  }
+
+  LW_DEV void finish_sums() {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+    }
+  }
+
+  // The piece to shared memory: accumulator, maximum and sum of every row.
+  LW_DEV void store_piece(float* piece, int lane) const {
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float* row = piece + (g + 8 * r) * S::kStride;
+#pragma unroll
+      for (int i = 0; i < HD / 8; ++i)
+        *reinterpret_cast<float2*>(row + i * 8 + 2 * t) = make_float2(o[i][2 * r], o[i][2 * r + 1]);
+      if (t == 0) {
+        row[HD] = m[r];
+        row[HD + 1] = l[r];
+      }
+    }
+  }
+
+  LW_DEV void store_out(const PagedDecodeParams& p, int b, int head0, int rows, int lane) const {
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (g + 8 * r >= rows) continue;
+      const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
+      T* dst = static_cast<T*>(p.out) + b * p.o_b + (long long)(head0 + g + 8 * r) * p.o_h + 2 * t;
+#pragma unroll
+      for (int i = 0; i < HD / 8; ++i)
+        *reinterpret_cast<uint32_t*>(dst + i * 8) = Elem<T>::pack(o[i][2 * r] * inv, o[i][2 * r + 1] * inv);
+    }
+  }
+};
+
+// The warp's copy of a tile into a ring stage: zeros for keys nobody sees.
+template <typename T, int HD, int ROWS>
+LW_DEV void copy_tile(const PagedDecodeParams& p, const TileSpan& sp, int key0, int page, int kvh, uint32_t dst,
+                      int lane) {
+  using S = DecodeShape<HD, ROWS>;
+  constexpr int CPR = HD / 8, ROWS_PER_INSTR = 32 / CPR, COPIES = kPdTile / ROWS_PER_INSTR;
+  const int c_row = lane / CPR, c_chunk = lane % CPR;
+  const int slot0 = key0 & (p.c.page_size - 1);
+  const T* kp = static_cast<const T*>(p.c.k) + page * p.c.kp + kvh * p.c.kh + slot0 * p.c.ks + c_chunk * 8;
+  const T* vp = static_cast<const T*>(p.c.v) + page * p.c.vp + kvh * p.c.vh + slot0 * p.c.vs + c_chunk * 8;
+#pragma unroll
+  for (int i = 0; i < COPIES; ++i) {
+    const int r = c_row + i * ROWS_PER_INSTR, key = key0 + r;
+    const bool ok = page >= 0 && key < sp.len && (key >= sp.lo || key < sp.sinks);
+    const uint32_t at = dst + (uint32_t)(r * (HD * 2) + ((c_chunk ^ (r & 7)) << 4));
+    cp_async16(at, ok ? kp + r * p.c.ks : static_cast<const T*>(p.q), ok);
+    cp_async16(at + S::kTileBytes, ok ? vp + r * p.c.vs : static_cast<const T*>(p.q), ok);
+  }
+}
+
+// A place on the line of tiles: sequence b, its span, item (kv head, head block) within it.
 struct LineCursor {
-  int b, hh;            // hh: (kv head, head block) within the sequence
+  int b, hh;
   long long item0;      // first tile of the item on the line
   TileSpan span;
 };
 
-template <typename T, int HD>
+template <typename T, int HD, int ROWS>
 __global__ void __launch_bounds__(kPdThreads, 1) paged_decode_kernel(const PagedDecodeParams p) {
-  constexpr int CPR = HD / 8;                      // 16-byte chunks per row
-  constexpr int kTileBytes = kPdTile * HD * 2;     // K or V of a tile
-  constexpr int kStages = 24576 / (2 * kTileBytes);   // 24 KB of ring per warp: 3 stages (hd 128), 6 (hd 64)
-  constexpr int ROWS_PER_INSTR = 32 / CPR;         // rows one cp.async of the warp covers
-  constexpr int COPIES = kPdTile / ROWS_PER_INSTR;
+  using S = DecodeShape<HD, ROWS>;
   extern __shared__ __align__(128) uint8_t smem[];
-  float* sm_o = reinterpret_cast<float*>(smem + kPdWarps * kStages * 2 * kTileBytes);   // [warps][8][HD]
-  __shared__ float sm_m[kPdWarps][kPdRows], sm_l[kPdWarps][kPdRows];
   __shared__ long long sm_scan[kPdWarps];
-  __shared__ long long sm_first;   // tiles before sm_b
-  __shared__ int sm_b;
+  __shared__ long long sm_first[kPdWarps];   // tiles before sm_b
+  __shared__ int sm_b[kPdWarps];
+  // pieces of items that do not lie in one run: entry 2w the one warp w's run
+  // begins in, entry 2w + 1 the one it ends in
+  __shared__ int sm_item[2 * kPdWarps], sm_runs[2 * kPdWarps];   // item or -1; CTAs its rest covers (0: it ends here)
+  __shared__ int sm_b_of[2 * kPdWarps];
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int H = p.c.nkv * p.hblocks;
+  float* head_piece = reinterpret_cast<float*>(smem + kPdWarps * S::kRing) + warp * S::kPiece;
+  float* tail_piece = reinterpret_cast<float*>(smem + warp * S::kRing);   // the ring, once it is drained
+  static_assert(S::kPiece * 4 <= S::kRing, "a piece fits in the ring");
   pdl_wait();
   pdl_launch_dependents();
 
-  // ---- this CTA's run of the line: a scan of the sequences' tile counts
+  // ---- the warps' runs of the line: a scan of the sequences' tile counts
   const int per_thread = (p.c.B + kPdThreads - 1) / kPdThreads;
   const int b_lo = min(p.c.B, tid * per_thread), b_hi = min(p.c.B, b_lo + per_thread);
   long long mine = 0;
@@ -98,6 +280,7 @@ __global__ void __launch_bounds__(kPdThreads, 1) paged_decode_kernel(const Paged
     if (lane >= o) incl += v;
   }
   if (lane == 31) sm_scan[warp] = incl;
+  if (tid < 2 * kPdWarps) sm_item[tid] = -1;
   __syncthreads();
   long long total = 0, before = 0;
 #pragma unroll
@@ -105,274 +288,307 @@ __global__ void __launch_bounds__(kPdThreads, 1) paged_decode_kernel(const Paged
     if (w < warp) before += sm_scan[w];
     total += sm_scan[w];
   }
-  long long run = (total + p.grid - 1) / p.grid;
-  if (run < kPdMinRun) run = kPdMinRun;
-  const long long r0 = blockIdx.x * run, r1 = min(total, r0 + run);
-  if (r0 >= r1) return;   // the whole CTA
-  {
-    long long excl = before + incl - mine;
-    if (mine > 0 && excl <= r0 && r0 < excl + mine) {
+  const long long lanes_of_work = (long long)gridDim.x * kPdWarps;
+  const long long run = max(1ll, (total + lanes_of_work - 1) / lanes_of_work);
+  const long long cta0 = (long long)blockIdx.x * kPdWarps * run;
+  if (cta0 >= total) return;   // the whole CTA
+  if (mine > 0) {
+    const long long mine0 = before + incl - mine;
+    for (int w = 0; w < kPdWarps; ++w) {
+      const long long at = cta0 + w * run;
+      if (at < mine0 || at >= mine0 + mine) continue;
+      long long excl = mine0;
       int b = b_lo;
       for (; b < b_hi - 1; ++b) {
         const long long n = (long long)tile_span(p, seq_len(p.c, b)).nt * H;
-        if (r0 < excl + n) break;
+        if (at < excl + n) break;
         excl += n;
       }
-      sm_b = b;
-      sm_first = excl;
+      sm_b[w] = b;
+      sm_first[w] = excl;
     }
   }
   __syncthreads();
 
-  LineCursor start;
-  start.b = sm_b;
-  start.span = tile_span(p, seq_len(p.c, start.b));
-  start.hh = (int)((r0 - sm_first) / start.span.nt);
-  start.item0 = sm_first + (long long)start.hh * start.span.nt;
-  auto advance = [&](LineCursor& c) {   // to the next item with tiles (one exists while its first tile < total)
-    c.item0 += c.span.nt;
-    if (++c.hh == H) {
-      c.hh = 0;
-      do {
-        ++c.b;
-        c.span = tile_span(p, seq_len(p.c, c.b));
-      } while (c.span.nt == 0);
-    }
-  };
+  const long long r0 = cta0 + warp * run, r1 = min(total, r0 + run);
+  if (r0 < r1) {
+    LineCursor cur;
+    cur.b = sm_b[warp];
+    cur.span = tile_span(p, seq_len(p.c, cur.b));
+    cur.hh = (int)((r0 - sm_first[warp]) / cur.span.nt);
+    cur.item0 = sm_first[warp] + (long long)cur.hh * cur.span.nt;
+    auto advance = [&](LineCursor& c) {   // to the next item with tiles (one exists while its first tile < total)
+      c.item0 += c.span.nt;
+      if (++c.hh == H) {
+        c.hh = 0;
+        do {
+          ++c.b;
+          c.span = tile_span(p, seq_len(p.c, c.b));
+        } while (c.span.nt == 0);
+      }
+    };
+    const uint32_t ring = smem_u32(smem) + warp * S::kRing;
+    LineCursor ahead = cur;
+    uint32_t lost = 0;   // bit st: the stage's page id was outside the pool, its keys are hidden
+    auto issue = [&](long long tile, int st) {
+      if (tile < r1) {
+        if (tile >= ahead.item0 + ahead.span.nt) advance(ahead);
+        const int key0 = ahead.span.key0((int)(tile - ahead.item0));
+        const int page = page_id(p.c, ahead.b, key0);
+        lost = page < 0 ? lost | (1u << st) : lost & ~(1u << st);
+        copy_tile<T, HD, ROWS>(p, ahead.span, key0, page, ahead.hh / p.hblocks, ring + st * (2 * S::kTileBytes), lane);
+      }
+      cp_async_commit();   // one group per call, empty past the run's end
+    };
+    long long next = r0;   // next tile to copy
+#pragma unroll
+    for (int s = 0; s < S::kStages; ++s) issue(next++, s);
 
-  // ---- the warp's copies: tile `tile` of the line into ring stage `st`
-  const uint32_t ring = smem_u32(smem) + warp * (kStages * 2 * kTileBytes);
-  const int c_row = lane / CPR, c_chunk = lane % CPR;
-  LineCursor ahead = start;
-  uint32_t lost = 0;   // bit st: the stage's page id was outside the pool, its keys are hidden
-  auto issue = [&](long long tile, int st) {
-    lost &= ~(1u << st);
-    if (tile < r1) {
-      while (tile >= ahead.item0 + ahead.span.nt) advance(ahead);
-      const int ti = (int)(tile - ahead.item0);
-      const TileSpan& sp = ahead.span;
-      const int key0 = (ti < sp.ns ? ti : sp.w0 + ti - sp.ns) * kPdTile;
-      const int page = page_id(p.c, ahead.b, key0);
-      const int slot0 = key0 & (p.c.page_size - 1);
-      if (page < 0) lost |= 1u << st;
-      const int kvh = ahead.hh / p.hblocks;
-      const T* kp = static_cast<const T*>(p.c.k) + page * p.c.kp + kvh * p.c.kh + slot0 * p.c.ks + c_chunk * 8;
-      const T* vp = static_cast<const T*>(p.c.v) + page * p.c.vp + kvh * p.c.vh + slot0 * p.c.vs + c_chunk * 8;
-      const uint32_t dst = ring + st * (2 * kTileBytes);
-#pragma unroll
-      for (int i = 0; i < COPIES; ++i) {
-        const int r = c_row + i * ROWS_PER_INSTR, key = key0 + r;
-        const bool ok = page >= 0 && key < sp.len && (key >= sp.lo || key < sp.sinks);
-        const uint32_t at = dst + (uint32_t)(r * (HD * 2) + ((c_chunk ^ (r & 7)) << 4));
-        cp_async16(at, ok ? kp + r * p.c.ks : static_cast<const T*>(p.q), ok);
-        cp_async16(at + kTileBytes, ok ? vp + r * p.c.vs : static_cast<const T*>(p.q), ok);
+    using Item = WarpItem<T, HD, ROWS>;
+    Item w;
+    auto head_of = [&](const LineCursor& c) {
+      const int kvh = c.hh / p.hblocks;
+      return kvh * p.group + (c.hh - kvh * p.hblocks) * ROWS;
+    };
+    auto rows_of = [&](const LineCursor& c) { return min(ROWS, p.group - c.hh % p.hblocks * ROWS); };
+    Item::load_q(p, cur.b, head_of(cur), rows_of(cur), lane, w.qa);
+    long long tile = r0;
+    int st = 0;
+    for (;;) {
+      const long long end = min(cur.item0 + cur.span.nt, r1);
+      const bool starts = cur.item0 >= r0, ends = cur.item0 + cur.span.nt <= r1;
+      LineCursor nxt = cur;
+      uint32_t qn[HD / 16][2 * Item::R];   // the next item's queries arrive meanwhile
+      if (end < r1) {
+        advance(nxt);
+        Item::load_q(p, nxt.b, head_of(nxt), rows_of(nxt), lane, qn);
       }
-    }
-    cp_async_commit();   // one group per call, empty past the run's end
-  };
-  long long next = r0 + warp;   // next tile to issue
-#pragma unroll
-  for (int s = 0; s < kStages; ++s, next += kPdWarps) issue(next, s);
-
-  // ---- items of the run
-  LineCursor cur = start;
-  long long tile = r0 + warp;
-  int st = 0;
-  for (;;) {
-    const long long seg0 = max(cur.item0, r0), seg1 = min(cur.item0 + cur.span.nt, r1);
-    const int kvh = cur.hh / p.hblocks, hb = cur.hh - kvh * p.hblocks;
-    const int rows = min(kPdRows, p.group - hb * kPdRows);
-    const int head0 = kvh * p.group + hb * kPdRows;
-
-    uint32_t qa[HD / 16][4];
-    {
-      const T* qp = static_cast<const T*>(p.q) + cur.b * p.q_b + (long long)head0 * p.q_h + 2 * t;
-#pragma unroll
-      for (int k = 0; k < HD / 16; ++k) {
-        qa[k][0] = g < rows ? *reinterpret_cast<const uint32_t*>(qp + g * p.q_h + k * 16) : 0u;
-        qa[k][2] = g < rows ? *reinterpret_cast<const uint32_t*>(qp + g * p.q_h + k * 16 + 8) : 0u;
-        qa[k][1] = g + 8 < rows ? *reinterpret_cast<const uint32_t*>(qp + (g + 8) * p.q_h + k * 16) : 0u;
-        qa[k][3] = g + 8 < rows ? *reinterpret_cast<const uint32_t*>(qp + (g + 8) * p.q_h + k * 16 + 8) : 0u;
+      w.clear();
+      for (; tile < end; ++tile) {
+        cp_async_wait<S::kStages - 1>();   // the oldest group has landed
+        __syncwarp();
+        w.tile(p, cur.span, cur.span.key0((int)(tile - cur.item0)), !((lost >> st) & 1u),
+               ring + st * (2 * S::kTileBytes), lane);
+        __syncwarp();   // every lane has read the stage
+        issue(next++, st);
+        if (++st == S::kStages) st = 0;
       }
-    }
-    float o[HD / 8][4];
-#pragma unroll
-    for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};   // rows g, g + 8
-
-    for (; tile < seg1; tile += kPdWarps) {
-      cp_async_wait<kStages - 1>();   // the oldest group has landed
-      __syncwarp();
-      const uint32_t kt = ring + st * (2 * kTileBytes), vt = kt + kTileBytes;
-      const int ti = (int)(tile - cur.item0);
-      const TileSpan& sp = cur.span;
-      const int key0 = (ti < sp.ns ? ti : sp.w0 + ti - sp.ns) * kPdTile;
-      const bool kept = !((lost >> st) & 1u);
-      auto sees = [&](int key) { return kept && key < sp.len && (key >= sp.lo || key < sp.sinks); };
-      float sc[2][4] = {};
-      {
-        // matrices of 8 keys x 8 dims: (keys 0-7 | 8-15) x (dims 0-7 | 8-15) of a k-step
-        const int r = (lane >> 4) * 8 + (lane & 7), cb = (lane >> 3) & 1;
-#pragma unroll
-        for (int k = 0; k < HD / 16; ++k) {
-          uint32_t b[4];
-          ldmatrix_x4(kt + (uint32_t)(r * (HD * 2) + (((2 * k + cb) ^ (r & 7)) << 4)), b);
-          mma_16816<T>(sc[0], qa[k][0], qa[k][1], qa[k][2], qa[k][3], b[0], b[1]);
-          mma_16816<T>(sc[1], qa[k][0], qa[k][1], qa[k][2], qa[k][3], b[2], b[3]);
+      w.finish_sums();
+      const int item = cur.b * H + cur.hh;
+      if (starts && ends) {
+        w.store_out(p, cur.b, head_of(cur), rows_of(cur), lane);
+        if (lane == 0) p.meta[item] = make_int2(0, 0);
+      } else {
+        const int e = 2 * warp + (starts ? 1 : 0);
+        if (lane == 0) {
+          sm_item[e] = item;
+          sm_b_of[e] = cur.b;
+          // CTAs after this one that hold tiles of the item
+          sm_runs[e] = (int)((cur.item0 + cur.span.nt - 1) / (run * kPdWarps) - blockIdx.x);
         }
-      }
-      float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int key = key0 + n * 8 + 2 * t + (e & 1);
-          sc[n][e] = sees(key) ? sc[n][e] * p.scale_log2 : -INFINITY;
-          mx[e >> 1] = fmaxf(mx[e >> 1], sc[n][e]);
-        }
-      float corr[2], base[2];
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-        const float mn = fmaxf(m[r], mx[r]);
-        corr[r] = m[r] == -INFINITY ? 0.f : exp2f(m[r] - mn);   // nothing summed yet: nothing to keep
-        base[r] = mn == -INFINITY ? 0.f : mn;   // no key seen yet: every weight is 0
-        m[r] = mn;
-        l[r] *= corr[r];
-      }
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          sc[n][e] = exp2f(sc[n][e] - base[e >> 1]);
-          l[e >> 1] += sc[n][e];
-        }
-      // the weights lie in [0, 1]: rounded to T for the second product, half a
-      // step each, averaged over the keys; their sum stays in fp32
-      const uint32_t a0 = Elem<T>::pack(sc[0][0], sc[0][1]), a1 = Elem<T>::pack(sc[0][2], sc[0][3]);
-      const uint32_t a2 = Elem<T>::pack(sc[1][0], sc[1][1]), a3 = Elem<T>::pack(sc[1][2], sc[1][3]);
-#pragma unroll
-      for (int i = 0; i < HD / 8; ++i) {
-        o[i][0] *= corr[0];
-        o[i][1] *= corr[0];
-        o[i][2] *= corr[1];
-        o[i][3] *= corr[1];
-      }
-      {
-        const int r = ((lane >> 3) & 1) * 8 + (lane & 7), cb = lane >> 4;
-#pragma unroll
-        for (int d = 0; d < HD / 16; ++d) {
-          uint32_t b[4];
-          ldmatrix_x4_t(vt + (uint32_t)(r * (HD * 2) + (((2 * d + cb) ^ (r & 7)) << 4)), b);
-          mma_16816<T>(o[2 * d], a0, a1, a2, a3, b[0], b[1]);
-          mma_16816<T>(o[2 * d + 1], a0, a1, a2, a3, b[2], b[3]);
-        }
-      }
-      __syncwarp();   // every lane has read the stage
-      issue(next, st);
-      next += kPdWarps;
-      if (++st == kStages) st = 0;
-    }
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-    }
-
-    // ---- the item's end in this run: the warps merge, eight rows at a time
-    const bool whole = seg0 == cur.item0 && seg1 == cur.item0 + cur.span.nt;
-    const int item = cur.b * H + cur.hh;
-    const bool head_slot = seg0 == r0;
-    float* slot = p.part + (long long)(2 * blockIdx.x + (head_slot ? 0 : 1)) * kPdRows * (HD + 2);
-    if (tid == 0 && seg0 == cur.item0) {
-      const long long last = (cur.item0 + cur.span.nt - 1) / run;
-      p.meta[item] = make_int2((int)blockIdx.x * 2 + (head_slot ? 0 : 1), whole ? 0 : (int)(last - blockIdx.x) + 1);
-    }
-    if (t == 0) {
-      sm_m[warp][g] = m[0];
-      sm_m[warp][g + 8] = m[1];
-      sm_l[warp][g] = l[0];
-      sm_l[warp][g + 8] = l[1];
-    }
-    for (int half = 0; half < 2 && half * 8 < rows; ++half) {
-      float* mine_o = sm_o + (warp * 8 + g) * HD + 2 * t;
-#pragma unroll
-      for (int i = 0; i < HD / 8; ++i)
-        *reinterpret_cast<float2*>(mine_o + i * 8) =
-            half ? make_float2(o[i][2], o[i][3]) : make_float2(o[i][0], o[i][1]);
-      __syncthreads();
-      const int n = min(8, rows - half * 8);
-      for (int i = tid; i < n * (HD / 2); i += kPdThreads) {
-        const int r = i / (HD / 2), d = (i - r * (HD / 2)) * 2, row = half * 8 + r;
-        float M = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < kPdWarps; ++w) M = fmaxf(M, sm_m[w][row]);
-        float L = 0.f, x = 0.f, y = 0.f;
-#pragma unroll
-        for (int w = 0; w < kPdWarps; ++w) {
-          const float f = sm_m[w][row] == -INFINITY ? 0.f : exp2f(sm_m[w][row] - M);   // a warp without tiles adds nothing
-          const float2 v = *reinterpret_cast<const float2*>(sm_o + (w * 8 + r) * HD + d);
-          L = fmaf(sm_l[w][row], f, L);
-          x = fmaf(v.x, f, x);
-          y = fmaf(v.y, f, y);
-        }
-        if (whole) {
-          T* dst = static_cast<T*>(p.out) + cur.b * p.o_b + (long long)(head0 + row) * p.o_h + d;
-          *reinterpret_cast<uint32_t*>(dst) = L == 0.f ? 0u : Elem<T>::pack(x / L, y / L);
+        if (starts) {
+          cp_async_wait<0>();   // the run's last item: the ring is drained
+          __syncwarp();
+          w.store_piece(tail_piece, lane);
         } else {
-          float* dst = slot + row * (HD + 2);
-          *reinterpret_cast<float2*>(dst + 2 + d) = make_float2(x, y);
-          if (d == 0) {
-            dst[0] = M;
-            dst[1] = L;
-          }
+          w.store_piece(head_piece, lane);
         }
       }
-      __syncthreads();   // the buffers are free again
+      if (end == r1) break;
+      cur = nxt;
+#pragma unroll
+      for (int k = 0; k < HD / 16; ++k)
+#pragma unroll
+        for (int r = 0; r < 2 * Item::R; ++r) w.qa[k][r] = qn[k][r];
     }
-    if (seg1 == r1) break;
-    advance(cur);
+  }
+  __syncthreads();
+
+  // ---- pieces of one item follow one another in the entries
+  for (int e = 0; e < 2 * kPdWarps;) {
+    const int item = sm_item[e];
+    if (item < 0) {
+      ++e;
+      continue;
+    }
+    int end = e + 1;
+    while (end < 2 * kPdWarps && (sm_item[end] < 0 || sm_item[end] == item)) ++end;
+    const int b = sm_b_of[e], hh = item - b * H, kvh = hh / p.hblocks, hb = hh - kvh * p.hblocks;
+    const int rows = min(ROWS, p.group - hb * ROWS);
+    const int more = sm_runs[e];
+    const bool starts = e & 1;
+    if (tid == 0 && starts) p.meta[item] = make_int2((int)blockIdx.x, more ? more + 1 : 0);
+    float* slot = p.part + (long long)(2 * blockIdx.x + (starts ? 1 : 0)) * S::kPiece;
+    auto piece = [&](int i) {
+      return reinterpret_cast<const float*>(smem + ((i & 1) ? (i >> 1) * S::kRing : kPdWarps * S::kRing +
+                                                                                        (i >> 1) * S::kPiece * 4));
+    };
+    for (int i = tid; i < rows * (HD / 2); i += kPdThreads) {
+      const int r = i / (HD / 2), d = (i - r * (HD / 2)) * 2;
+      float M = -INFINITY;
+      for (int x = e; x < end; ++x)
+        if (sm_item[x] >= 0) M = fmaxf(M, piece(x)[r * S::kStride + HD]);
+      float L = 0.f, x0 = 0.f, x1 = 0.f;
+      for (int x = e; x < end; ++x) {
+        if (sm_item[x] < 0) continue;
+        const float* row = piece(x) + r * S::kStride;
+        const float f = row[HD] == -INFINITY ? 0.f : ex2(row[HD] - M);   // no key seen in this piece
+        const float2 v = *reinterpret_cast<const float2*>(row + d);
+        L = fmaf(row[HD + 1], f, L);
+        x0 = fmaf(v.x, f, x0);
+        x1 = fmaf(v.y, f, x1);
+      }
+      if (starts && !more) {
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        T* dst = static_cast<T*>(p.out) + b * p.o_b + (long long)(kvh * p.group + hb * ROWS + r) * p.o_h + d;
+        *reinterpret_cast<uint32_t*>(dst) = Elem<T>::pack(x0 * inv, x1 * inv);
+      } else {
+        float* dst = slot + r * S::kStride;
+        *reinterpret_cast<float2*>(dst + d) = make_float2(x0, x1);
+        if (d == 0) *reinterpret_cast<float2*>(dst + HD) = make_float2(M, L);
+      }
+    }
+    e = end;
   }
 }
 
-// Joins the runs of every item that was split, in the order of the line, and
-// writes zeros for sequences without a visible key. One block per item.
-template <typename T, int HD>
+// Joins the pieces of every item that several CTAs hold, in the order of the
+// line, and writes zeros for sequences without a visible key. One block per item.
+template <typename T, int HD, int ROWS>
 __global__ void __launch_bounds__(HD) paged_join_kernel(const PagedDecodeParams p) {
+  using S = DecodeShape<HD, ROWS>;
   pdl_wait();
   pdl_launch_dependents();
   const int H = p.c.nkv * p.hblocks;
   const int b = blockIdx.x / H, hh = blockIdx.x - b * H;
   const int kvh = hh / p.hblocks, hb = hh - kvh * p.hblocks;
-  const int rows = min(kPdRows, p.group - hb * kPdRows);
-  T* dst = static_cast<T*>(p.out) + b * p.o_b + (long long)(kvh * p.group + hb * kPdRows) * p.o_h;
+  const int rows = min(ROWS, p.group - hb * ROWS);
+  T* dst = static_cast<T*>(p.out) + b * p.o_b + (long long)(kvh * p.group + hb * ROWS) * p.o_h;
   const int d = (threadIdx.x % (HD / 2)) * 2;
   if (seq_len(p.c, b) == 0) {
     for (int r = threadIdx.x / (HD / 2); r < rows; r += 2) *reinterpret_cast<uint32_t*>(dst + r * p.o_h + d) = 0u;
     return;
   }
   const int2 mt = p.meta[blockIdx.x];
-  if (mt.y == 0) return;   // written by the one run that holds it
+  if (mt.y == 0) return;   // written by the one CTA that holds it
   for (int r = threadIdx.x / (HD / 2); r < rows; r += 2) {
-    auto slot = [&](int i) {
-      const int s = i == 0 ? mt.x : 2 * ((mt.x >> 1) + i);
-      return p.part + ((long long)s * kPdRows + r) * (HD + 2);
+    auto row = [&](int i) {
+      return p.part + (long long)(i == 0 ? 2 * mt.x + 1 : 2 * (mt.x + i)) * S::kPiece + r * S::kStride;
     };
     float M = -INFINITY;
-    for (int i = 0; i < mt.y; ++i) M = fmaxf(M, slot(i)[0]);
+#pragma unroll 8
+    for (int i = 0; i < mt.y; ++i) M = fmaxf(M, row(i)[HD]);
     float L = 0.f, x = 0.f, y = 0.f;
-#pragma unroll 4
+#pragma unroll 8
     for (int i = 0; i < mt.y; ++i) {
-      const float* s = slot(i);
-      const float f = s[0] == -INFINITY ? 0.f : exp2f(s[0] - M);
-      const float2 v = *reinterpret_cast<const float2*>(s + 2 + d);
-      L = fmaf(s[1], f, L);
+      const float* s = row(i);
+      const float2 ml = *reinterpret_cast<const float2*>(s + HD);
+      const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
+      const float2 v = *reinterpret_cast<const float2*>(s + d);
+      L = fmaf(ml.y, f, L);
       x = fmaf(v.x, f, x);
       y = fmaf(v.y, f, y);
     }
-    *reinterpret_cast<uint32_t*>(dst + r * p.o_h + d) = L == 0.f ? 0u : Elem<T>::pack(x / L, y / L);
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    *reinterpret_cast<uint32_t*>(dst + r * p.o_h + d) = Elem<T>::pack(x * inv, y * inv);
   }
+}
+
+// An item per cluster: its CTAs' warps take the tiles in turn.
+template <typename T, int HD, int ROWS>
+__global__ void __launch_bounds__(kPdThreads, 1) paged_decode_cluster_kernel(const PagedDecodeParams p) {
+  namespace cg = cooperative_groups;
+  using S = DecodeShape<HD, ROWS>;
+  using Item = WarpItem<T, HD, ROWS>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  float* pieces = reinterpret_cast<float*>(smem + kPdWarps * S::kRing);
+  float* joined = reinterpret_cast<float*>(smem);   // this CTA's piece, once the rings are drained
+  cg::cluster_group cluster = cg::this_cluster();
+  const int CL = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int H = p.c.nkv * p.hblocks;
+  const int item = blockIdx.y, b = item / H, hh = item - b * H, kvh = hh / p.hblocks, hb = hh - kvh * p.hblocks;
+  const int head0 = kvh * p.group + hb * ROWS, rows = min(ROWS, p.group - hb * ROWS);
+  pdl_wait();
+  pdl_launch_dependents();
+  Item w;
+  Item::load_q(p, b, head0, rows, lane, w.qa);
+  const TileSpan sp = tile_span(p, seq_len(p.c, b));
+  const int step = CL * kPdWarps;
+  const uint32_t ring = smem_u32(smem) + warp * S::kRing;
+  uint32_t lost = 0;
+  auto issue = [&](int tile, int st) {
+    if (tile < sp.nt) {
+      const int key0 = sp.key0(tile), page = page_id(p.c, b, key0);
+      lost = page < 0 ? lost | (1u << st) : lost & ~(1u << st);
+      copy_tile<T, HD, ROWS>(p, sp, key0, page, kvh, ring + st * (2 * S::kTileBytes), lane);
+    }
+    cp_async_commit();
+  };
+  int tile = rank * kPdWarps + warp, next = tile, st = 0;
+#pragma unroll
+  for (int s = 0; s < S::kStages; ++s, next += step) issue(next, s);
+  w.clear();
+  for (; tile < sp.nt; tile += step) {
+    cp_async_wait<S::kStages - 1>();
+    __syncwarp();
+    w.tile(p, sp, sp.key0(tile), !((lost >> st) & 1u), ring + st * (2 * S::kTileBytes), lane);
+    __syncwarp();
+    issue(next, st);
+    next += step;
+    if (++st == S::kStages) st = 0;
+  }
+  w.finish_sums();
+  w.store_piece(pieces + warp * S::kPiece, lane);
+  cp_async_wait<0>();
+  __syncthreads();
+  for (int i = tid; i < rows * (HD / 2); i += kPdThreads) {
+    const int r = i / (HD / 2), d = (i - r * (HD / 2)) * 2;
+    const float* row = pieces + r * S::kStride;
+    float M = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < kPdWarps; ++x) M = fmaxf(M, row[x * S::kPiece + HD]);
+    float L = 0.f, x0 = 0.f, x1 = 0.f;
+#pragma unroll
+    for (int x = 0; x < kPdWarps; ++x) {
+      const float* s = row + x * S::kPiece;
+      const float f = s[HD] == -INFINITY ? 0.f : ex2(s[HD] - M);   // a warp without tiles adds nothing
+      L = fmaf(s[HD + 1], f, L);
+      x0 = fmaf(s[d], f, x0);
+      x1 = fmaf(s[d + 1], f, x1);
+    }
+    float* dst = joined + r * S::kStride;
+    *reinterpret_cast<float2*>(dst + d) = make_float2(x0, x1);
+    if (d == 0) *reinterpret_cast<float2*>(dst + HD) = make_float2(M, L);
+  }
+  cluster.sync();
+  for (int i = rank * kPdThreads + tid; i < rows * (HD / 2); i += CL * kPdThreads) {
+    const int r = i / (HD / 2), d = (i - r * (HD / 2)) * 2;
+    float2 ml[8], v[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {   // the remote reads together
+      const float* s = cluster.map_shared_rank(joined, c < CL ? c : 0) + r * S::kStride;
+      ml[c] = *reinterpret_cast<const float2*>(s + HD);
+      v[c] = *reinterpret_cast<const float2*>(s + d);
+    }
+    float M = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      if (c < CL) M = fmaxf(M, ml[c].x);
+    float L = 0.f, x0 = 0.f, x1 = 0.f;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      if (c >= CL) break;
+      const float f = ml[c].x == -INFINITY ? 0.f : ex2(ml[c].x - M);
+      L = fmaf(ml[c].y, f, L);
+      x0 = fmaf(v[c].x, f, x0);
+      x1 = fmaf(v[c].y, f, x1);
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    T* dst = static_cast<T*>(p.out) + b * p.o_b + (long long)(head0 + r) * p.o_h + d;
+    *reinterpret_cast<uint32_t*>(dst) = Elem<T>::pack(x0 * inv, x1 * inv);
+  }
+  cluster.sync();   // this CTA's shared memory lives until every remote read is done
 }
 
 }  // namespace lw
@@ -380,7 +596,7 @@ __global__ void __launch_bounds__(HD) paged_join_kernel(const PagedDecodeParams 
 namespace {
 
 struct DecodePlan {
-  int group, hblocks, grid;
+  int group, rows, hblocks, grid, cluster;   // cluster 0: runs and a join
   long long items;
   size_t part_off, bytes;
 };
@@ -388,23 +604,63 @@ struct DecodePlan {
 DecodePlan decode_plan(const lw_paged_attention_args* a) {
   DecodePlan d;
   d.group = a->n_q_heads / a->cache.n_kv_heads;
-  d.hblocks = (d.group + lw::kPdRows - 1) / lw::kPdRows;
+  d.rows = d.group <= 8 ? 8 : 16;
+  d.hblocks = (d.group + d.rows - 1) / d.rows;
   d.items = (long long)a->cache.batch * a->cache.n_kv_heads * d.hblocks;
   d.grid = lw_host::sm_count();
+  // Clusters of as many CTAs as the SMs hold beside each other (up to 8), when
+  // no sequence can give one of their CTAs more than 32 tiles (four per warp).
+  long long keys = (long long)a->cache.table_width * a->cache.page_size;
+  if (a->window > 0) keys = std::min(keys, (long long)a->window + a->sinks);
+  d.cluster = 8;
+  while (d.cluster > 1 && d.items * d.cluster > d.grid) d.cluster /= 2;
+  if (d.items * d.cluster > d.grid || keys > 32ll * lw::kPdTile * d.cluster) d.cluster = 0;
   d.part_off = ((size_t)d.items * sizeof(int2) + 255) & ~(size_t)255;
-  d.bytes = d.part_off + (size_t)2 * d.grid * lw::kPdRows * (a->cache.head_dim + 2) * sizeof(float);
+  d.bytes = d.cluster ? 0 : d.part_off + (size_t)2 * d.grid * d.rows * (a->cache.head_dim + 8) * sizeof(float);
   return d;
 }
 
-template <typename T, int HD>
-cudaError_t decode_launch(const lw::PagedDecodeParams& p, long long items, cudaStream_t s, bool pdl) {
-  constexpr int smem = lw::kPdWarps * 24576 + lw::kPdWarps * 8 * HD * (int)sizeof(float);
-  auto kern = lw::paged_decode_kernel<T, HD>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+template <typename Kernel>
+cudaError_t allow_smem(Kernel kern, int bytes) {
+  return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+
+template <typename T, int HD, int ROWS>
+cudaError_t decode_launch(const lw::PagedDecodeParams& p, const DecodePlan& d, cudaStream_t s, bool pdl) {
+  constexpr int smem = lw::DecodeShape<HD, ROWS>::kBytes;
+  if (d.cluster) {
+    auto kern = lw::paged_decode_cluster_kernel<T, HD, ROWS>;
+    cudaError_t e = allow_smem(kern, smem);
+    if (e != cudaSuccess) return e;
+    lw_count_launch();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)d.cluster, (unsigned)d.items);
+    cfg.blockDim = dim3(lw::kPdThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)d.cluster;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kern, p);
+  }
+  auto kern = lw::paged_decode_kernel<T, HD, ROWS>;
+  cudaError_t e = allow_smem(kern, smem);
   if (e != cudaSuccess) return e;
-  e = lw_launch(kern, dim3(p.grid), dim3(lw::kPdThreads), smem, s, pdl, p);
+  e = lw_launch(kern, dim3(d.grid), dim3(lw::kPdThreads), smem, s, pdl, p);
   if (e != cudaSuccess) return e;
-  return lw_launch(lw::paged_join_kernel<T, HD>, dim3((unsigned)items), dim3(HD), 0, s, true, p);
+  return lw_launch(lw::paged_join_kernel<T, HD, ROWS>, dim3((unsigned)d.items), dim3(HD), 0, s, true, p);
+}
+
+template <typename T>
+cudaError_t decode_dispatch(const lw::PagedDecodeParams& p, int hd, const DecodePlan& d, cudaStream_t s, bool pdl) {
+  if (hd == 128) return d.rows == 8 ? decode_launch<T, 128, 8>(p, d, s, pdl) : decode_launch<T, 128, 16>(p, d, s, pdl);
+  return d.rows == 8 ? decode_launch<T, 64, 8>(p, d, s, pdl) : decode_launch<T, 64, 16>(p, d, s, pdl);
 }
 
 }  // namespace
@@ -425,22 +681,15 @@ int lw_paged_decode(const lw_paged_attention_args* a, cudaStream_t s) {
   p.q_h = a->q_strides[1];
   p.o_b = a->out_strides[0];
   p.o_h = a->out_strides[1];
-  p.nq = a->n_q_heads;
   p.group = d.group;
   p.hblocks = d.hblocks;
   p.window = a->window;
   p.sinks = a->sinks;
   p.scale_log2 = a->scale * 1.4426950408889634f;
-  p.grid = d.grid;
   p.meta = static_cast<int2*>(a->workspace);
   p.part = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + d.part_off);
   const bool pdl = a->pdl != 0;
-  cudaError_t e;
-  if (a->cache.dtype == LW_DTYPE_F16)
-    e = a->cache.head_dim == 128 ? decode_launch<__half, 128>(p, d.items, s, pdl)
-                                 : decode_launch<__half, 64>(p, d.items, s, pdl);
-  else
-    e = a->cache.head_dim == 128 ? decode_launch<__nv_bfloat16, 128>(p, d.items, s, pdl)
-                                 : decode_launch<__nv_bfloat16, 64>(p, d.items, s, pdl);
+  const cudaError_t e = a->cache.dtype == LW_DTYPE_F16 ? decode_dispatch<__half>(p, a->cache.head_dim, d, s, pdl)
+                                                       : decode_dispatch<__nv_bfloat16>(p, a->cache.head_dim, d, s, pdl);
   return e == cudaSuccess ? LW_OK : LW_ERR_LAUNCH;
 }

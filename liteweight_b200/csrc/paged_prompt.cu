@@ -88,12 +88,6 @@ LW_DEV bool find_row_tile(const PromptParams& p, int slot, int& b, int& i0, int&
   return i0 >= 0 && i0 < n && o >= 0 && (long long)o + n <= p.T;
 }
 
-LW_DEV float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 template <int HD>
 struct PromptSmem {
   static constexpr int kTile = kPmKeys * HD * 2;              // a K, V or Q tile

@@ -28,6 +28,7 @@ output and scratch from torch, and can be captured in a CUDA graph.
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
@@ -36,7 +37,7 @@ from liteweight_b200 import _native as nat
 c_int, c_void_p, c_float, c_size_t, c_ll = (ctypes.c_int, ctypes.c_void_p, ctypes.c_float, ctypes.c_size_t,
                                             ctypes.c_longlong)
 _INT_MAX = 2**31 - 1
-_DTYPE = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_F16, _BF16, _F32, _I32 = torch.float16, torch.bfloat16, torch.float32, torch.int32
 
 
 class PagedCacheArgs(ctypes.Structure):
@@ -65,60 +66,71 @@ class PagedAttentionArgs(ctypes.Structure):
                 ("workspace", c_void_p), ("workspace_bytes", c_size_t)]
 
 
-nat.register("lw_qk_norm_rope", [ctypes.POINTER(QkNormRopeArgs), c_void_p])
-nat.register("lw_paged_attention", [ctypes.POINTER(PagedAttentionArgs), c_void_p])
-nat.register("lw_paged_attention_workspace_size", [ctypes.POINTER(PagedAttentionArgs)], c_size_t)
+# The calls below write the same structs with struct.pack (one call instead of a
+# ctypes object per field: a decode step makes two of them per layer). Native
+# alignment, so the layouts are the C compiler's.
+_CACHE_FMT = "PP6q6iPqi0qP"
+_ROPE = struct.Struct("@" + _CACHE_FMT + "PPP6qP2qii0qPPPqiiPPfii0q")
+_ATTN = struct.Struct("@" + _CACHE_FMT + "P2qP2qii0qPiifii0qPN")
+assert _ROPE.size == ctypes.sizeof(QkNormRopeArgs) and _ATTN.size == ctypes.sizeof(PagedAttentionArgs)
+
+nat.register("lw_qk_norm_rope", [c_void_p, c_void_p])
+nat.register("lw_paged_attention", [c_void_p, c_void_p])
+nat.register("lw_paged_attention_workspace_size", [c_void_p], c_size_t)
 
 
 def _rows(name: str, t: torch.Tensor, dtype: torch.dtype, hd: int) -> tuple[int, int]:
     """(token, head) strides of a [tokens, heads, head_dim] tensor."""
-    assert t.dtype == dtype, f"{name} is {t.dtype}, the cache {dtype}"
+    assert t.dtype is dtype, f"{name} is {t.dtype}, the cache {dtype}"
     assert t.dim() == 3 and t.shape[2] == hd, f"{name} must be [tokens, heads, {hd}], got {tuple(t.shape)}"
     st, sh, sd = t.stride()
     assert sd == 1 or t.numel() == 0, f"{name}'s last dimension must be contiguous"
     return st, sh
 
 
-def _cache_args(k_pages, v_pages, page_table, kv_lens) -> PagedCacheArgs:
-    assert k_pages.dtype in (torch.float16, torch.bfloat16) and v_pages.dtype == k_pages.dtype
-    assert k_pages.dim() == 4 and k_pages.shape == v_pages.shape, "k_pages / v_pages: [pages, kv heads, page, head_dim]"
-    assert page_table.dtype == torch.int32 and kv_lens.dtype == torch.int32, "page_table and kv_lens are int32"
-    assert page_table.dim() == 2 and kv_lens.dim() == 1 and page_table.shape[0] == kv_lens.shape[0]
-    kp, kh, ks, kd = k_pages.stride()
-    vp, vh, vs, vd = v_pages.stride()
-    batch, width = page_table.shape
-    ts, te = page_table.stride()
-    assert (kd == 1 and vd == 1) or k_pages.numel() == 0, "the pools' last dimension must be contiguous"
-    assert te == 1 or width <= 1, "page_table's rows must be contiguous"
-    assert kv_lens.stride(0) == 1 or batch <= 1, "kv_lens must be contiguous"
-    n_pages, n_kv, page, hd = k_pages.shape
-    return PagedCacheArgs(k_pages.data_ptr(), v_pages.data_ptr(), (kp, kh, ks), (vp, vh, vs), n_pages, page, n_kv, hd,
-                          _DTYPE[k_pages.dtype], batch, page_table.data_ptr(), ts, width, kv_lens.data_ptr())
+def _cache_fields(k_pages, v_pages, page_table, kv_lens) -> tuple:
+    dt = k_pages.dtype
+    assert (dt is _F16 or dt is _BF16) and v_pages.dtype is dt, "k_pages / v_pages: both float16 or both bfloat16"
+    shape = k_pages.shape
+    assert len(shape) == 4 and shape == v_pages.shape, "k_pages / v_pages: [pages, kv heads, page, head_dim]"
+    assert page_table.dtype is _I32 and kv_lens.dtype is _I32, "page_table and kv_lens are int32"
+    ks, vs, ts, tshape = k_pages.stride(), v_pages.stride(), page_table.stride(), page_table.shape
+    assert len(tshape) == 2 and kv_lens.shape == tshape[:1], "page_table: [batch, width], kv_lens: [batch]"
+    batch, width = tshape
+    assert (ks[3] == 1 and vs[3] == 1) or k_pages.numel() == 0, "the pools' last dimension must be contiguous"
+    assert ts[1] == 1 or width <= 1, "page_table's rows must be contiguous"
+    assert batch <= 1 or kv_lens.stride(0) == 1, "kv_lens must be contiguous"
+    return (k_pages.data_ptr(), v_pages.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], shape[0], shape[2],
+            shape[1], shape[3], 0 if dt is _F16 else 1, batch, page_table.data_ptr(), ts[0], width, kv_lens.data_ptr())
 
 
-def _offsets(q_offsets, batch: int, tokens: int):
+def _offsets(q_offsets, batch: int, tokens: int) -> int:
     if q_offsets is None:
         assert tokens == batch, f"one new token per sequence: {tokens} rows for {batch} sequences"
-        return None
-    assert q_offsets.dtype == torch.int32 and q_offsets.shape == (batch + 1,), f"q_offsets: int32 [{batch + 1}]"
+        return 0
+    assert q_offsets.dtype is _I32 and q_offsets.shape == (batch + 1,), f"q_offsets: int32 [{batch + 1}]"
     assert q_offsets.stride(0) == 1, "q_offsets must be contiguous"
     return q_offsets.data_ptr()
 
 
-def _same_device(*ts) -> torch.device:
-    nat.require_cuda(*ts)
-    dev = ts[0].device
+def _device_of(*ts) -> int:
+    """Index of the one device that holds them all."""
+    dev = ts[0].get_device()
     for t in ts:
-        assert t is None or t.device == dev, "all tensors must be on one device"
+        if t is not None and (dev < 0 or t.get_device() != dev):
+            nat.require_cuda(*ts)
+            raise AssertionError("all tensors must be on one device")
     return dev
 
 
-def _run(fn: str, args, dev: torch.device) -> None:
-    if torch.cuda.current_device() == dev.index:
-        nat.call(fn, ctypes.byref(args), torch.cuda.current_stream(dev).cuda_stream)
+def _run(fn: str, args: bytes, dev: int) -> None:
+    if torch.cuda.current_device() == dev:
+        status = getattr(nat.lib(), fn)(args, torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
-            nat.call(fn, ctypes.byref(args), torch.cuda.current_stream(dev).cuda_stream)
+            status = getattr(nat.lib(), fn)(args, torch._C._cuda_getCurrentRawStream(dev))
+    if status:
+        nat.check(fn, status)
 
 
 def check_device_error() -> None:
@@ -153,53 +165,60 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.T
     q_offsets[-1] on) are zero, or left as they were in a given `out`. New tokens
     must not share a slot.
     """
-    cache = _cache_args(k_pages, v_pages, page_table, kv_lens)
-    dt, hd = k_pages.dtype, cache.head_dim
+    cache = _cache_fields(k_pages, v_pages, page_table, kv_lens)
+    dt, nkv, hd, batch = k_pages.dtype, cache[10], cache[11], cache[13]
     qs, ks, vs = _rows("q", q, dt, hd), _rows("k", k, dt, hd), _rows("v", v, dt, hd)
-    T, nq = q.shape[0], q.shape[1]
-    assert k.shape[0] == T and k.shape[1] == cache.n_kv_heads and v.shape == k.shape
-    assert cos.dim() == 2 and cos.shape[1] == hd and cos.shape == sin.shape and cos.dtype == sin.dtype
-    assert cos.dtype in (dt, torch.float32), f"cos / sin: {dt} or float32"
-    assert cos.stride() == sin.stride() and (cos.stride(1) == 1 or cos.numel() == 0)
+    T, nq, _ = q.shape
+    assert k.shape == (T, nkv, hd) and v.shape == k.shape, f"k and v: [{T}, {nkv}, {hd}]"
+    tt, tshape, ts = cos.dtype, cos.shape, cos.stride()
+    assert len(tshape) == 2 and tshape[1] == hd and tshape == sin.shape, f"cos / sin: [positions, {hd}]"
+    assert (tt is dt or tt is _F32) and sin.dtype is tt, f"cos / sin: {dt} or float32"
+    assert ts == sin.stride() and (ts[1] == 1 or cos.numel() == 0), "cos / sin: rows contiguous, strides alike"
     assert (q_weight is None) == (k_weight is None), "norm weights for both queries and keys, or for neither"
-    for w in (q_weight, k_weight):
-        assert w is None or (w.dtype == dt and w.shape == (hd,) and w.stride(0) == 1)
-    off = _offsets(q_offsets, cache.batch, T)
+    if q_weight is not None:
+        for w in (q_weight, k_weight):
+            assert w.dtype is dt and w.shape == (hd,) and w.stride(0) == 1, f"norm weights: {dt} [{hd}]"
+    off = _offsets(q_offsets, batch, T)
     assert out is None or out.shape == q.shape, "out must have q's shape"
-    dev = _same_device(q, k, v, cos, sin, k_pages, v_pages, page_table, kv_lens, q_offsets, q_weight, k_weight, out)
+    dev = _device_of(q, k, v, cos, sin, k_pages, v_pages, page_table, kv_lens, q_offsets, q_weight, k_weight, out)
     fresh = out is None
     if fresh:
-        out = torch.empty((T, nq, hd), dtype=dt, device=dev)
-    os_ = _rows("out", out, dt, hd)
-    _run("lw_qk_norm_rope", QkNormRopeArgs(
-        cache, q.data_ptr(), k.data_ptr(), v.data_ptr(), qs, ks, vs, out.data_ptr(), os_, T, nq, off, cos.data_ptr(),
-        sin.data_ptr(), cos.stride(0), _DTYPE[cos.dtype], cos.shape[0], nat.ptr(q_weight), nat.ptr(k_weight), eps,
-        fresh, 1), dev)
+        out = torch.empty((T, nq, hd), dtype=dt, device=q.device)
+        os_ = (nq * hd, hd)
+    else:
+        os_ = _rows("out", out, dt, hd)
+    _run("lw_qk_norm_rope", _ROPE.pack(
+        *cache, q.data_ptr(), k.data_ptr(), v.data_ptr(), *qs, *ks, *vs, out.data_ptr(), *os_, T, nq, off,
+        cos.data_ptr(), sin.data_ptr(), ts[0], 2 if tt is _F32 else cache[12], tshape[0],
+        0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(), eps, fresh, 1),
+        dev)
     return out
 
 
 def _attention(q, k_pages, v_pages, page_table, kv_lens, q_offsets, window, sinks, scale, out):
-    cache = _cache_args(k_pages, v_pages, page_table, kv_lens)
-    dt, hd = k_pages.dtype, cache.head_dim
+    cache = _cache_fields(k_pages, v_pages, page_table, kv_lens)
+    dt, hd, batch = k_pages.dtype, cache[11], cache[13]
     qs = _rows("q", q, dt, hd)
-    T, nq = q.shape[0], q.shape[1]
-    assert nq % cache.n_kv_heads == 0, f"{nq} query heads over {cache.n_kv_heads} kv heads"
+    T, nq, _ = q.shape
+    assert nq % cache[10] == 0, f"{nq} query heads over {cache[10]} kv heads"
     assert window is None or window >= 1, "window: at least 1, or None"
-    assert sinks >= 0
-    off = _offsets(q_offsets, cache.batch, T)
-    assert out is None or (out.shape == q.shape and out.dtype == dt), "out must have q's shape and type"
-    dev = _same_device(q, k_pages, v_pages, page_table, kv_lens, q_offsets, out)
+    assert sinks >= 0, "sinks: at least 0"
+    off = _offsets(q_offsets, batch, T)
+    assert out is None or (out.shape == q.shape and out.dtype is dt), "out must have q's shape and type"
+    dev = _device_of(q, k_pages, v_pages, page_table, kv_lens, q_offsets, out)
     fresh = out is None
     if fresh:
-        out = torch.empty((T, nq, hd), dtype=dt, device=dev)
-    os_ = _rows("out", out, dt, hd)
-    args = PagedAttentionArgs(cache, q.data_ptr(), qs, out.data_ptr(), os_, T, nq, off, min(window or 0, _INT_MAX),
-                              min(sinks, _INT_MAX),
-                              hd ** -0.5 if scale is None else scale, fresh, 1, None, 0)
-    need = nat.lib().lw_paged_attention_workspace_size(ctypes.byref(args))
+        out = torch.empty((T, nq, hd), dtype=dt, device=q.device)
+        os_ = (nq * hd, hd)
+    else:
+        os_ = _rows("out", out, dt, hd)
+    fields = (*cache, q.data_ptr(), *qs, out.data_ptr(), *os_, T, nq, off, min(window or 0, _INT_MAX),
+              min(sinks, _INT_MAX), hd ** -0.5 if scale is None else scale, fresh, 1)
+    args = _ATTN.pack(*fields, 0, 0)
+    need = nat.lib().lw_paged_attention_workspace_size(args)
     if need:   # scratch of this call alone: calls on other streams or in other graphs never share it
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        args.workspace, args.workspace_bytes = ws.data_ptr(), need
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        args = _ATTN.pack(*fields, ws.data_ptr(), need)
     _run("lw_paged_attention", args, dev)
     return out
 

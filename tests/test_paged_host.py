@@ -42,6 +42,8 @@ def rope_args(cache=None, **kw):
     return paged.QkNormRopeArgs(**d)
 
 
+LONG = cache_args(table_width=1 << 16, table_stride=1 << 16)   # long enough that its decode needs scratch
+
 BAD_CACHE = [
     (dict(page_size=24), 2), (dict(page_size=0), 2), (dict(page_size=8), 5), (dict(page_size=512), 5),
     (dict(head_dim=80), 5), (dict(dtype=2), 5), (dict(dtype=7), 5), (dict(n_kv_heads=0), 2), (dict(batch=-1), 2),
@@ -63,8 +65,8 @@ def test_bad_caches_are_refused(lib, kw, status):
     (dict(q=None), 1), (dict(out=None), 1), (dict(tokens=3), 2), (dict(n_q_heads=6), 2), (dict(n_q_heads=0), 2),
     (dict(sinks=-1), 2), (dict(scale=0.0), 2), (dict(scale=-1.0), 2), (dict(scale=float("nan")), 2),
     (dict(scale=float("inf")), 2), (dict(q=FAKE + 8), 4), (dict(out_strides=(1024, 130)), 4), (dict(tokens=-1), 2),
-    (dict(workspace=None), 7), (dict(workspace=FAKE, workspace_bytes=256), 7),
-    (dict(workspace=FAKE + 16, workspace_bytes=1 << 30), 4),
+    (dict(cache=LONG, workspace=None), 7), (dict(cache=LONG, workspace=FAKE, workspace_bytes=256), 7),
+    (dict(cache=LONG, workspace=FAKE + 16, workspace_bytes=1 << 30), 4),
     (dict(q_offsets=FAKE + 2), 4), (dict(q_offsets=FAKE, n_q_heads=4 * 65), 5),
 ])
 def test_bad_attention_arguments_are_refused(lib, kw, status):
@@ -91,6 +93,20 @@ def test_empty_calls_do_nothing(lib):
 
 def test_status_string(lib):
     assert lib.lw_status_string(9) == b"page id, position or length out of range"
+
+
+@pytest.mark.parametrize("packer,mirror", [("_ROPE", "QkNormRopeArgs"), ("_ATTN", "PagedAttentionArgs")])
+def test_packed_arguments_are_the_struct(lib, packer, mirror):
+    def fields(s):
+        out = []
+        for name, _ in s._fields_:
+            v = getattr(s, name)
+            out += fields(v) if isinstance(v, ctypes.Structure) else list(v) if isinstance(v, ctypes.Array) else [v]
+        return out
+    cls, pack = getattr(paged, mirror), getattr(paged, packer)
+    values = list(range(1, len(fields(cls())) + 1))
+    assert fields(cls.from_buffer_copy(pack.pack(*values))) == values
+    assert lib.lw_struct_size(6 if packer == "_ROPE" else 7) == pack.size
 
 
 def tensors(**kw):
