@@ -45,7 +45,7 @@ struct PagedDecodeParams {
   int group, hblocks;       // group = query heads per kv head; hblocks = blocks of ROWS heads in it
   int window, sinks;
   float scale_log2;
-  int2* meta;               // [items]: first CTA, CTAs that hold a piece (0: nothing to join)
+  int2* meta;               // [grid]: the item that begins in this CTA and ends in another, CTAs that hold it (or 0)
   float* part;              // [2 * grid][ROWS][HD + 8]
 };
 
@@ -291,7 +291,10 @@ __global__ void __launch_bounds__(kPdThreads, 1) paged_decode_kernel(const Paged
   const long long lanes_of_work = (long long)gridDim.x * kPdWarps;
   const long long run = max(1ll, (total + lanes_of_work - 1) / lanes_of_work);
   const long long cta0 = (long long)blockIdx.x * kPdWarps * run;
-  if (cta0 >= total) return;   // the whole CTA
+  if (cta0 >= total) {   // the whole CTA
+    if (tid == 0) p.meta[blockIdx.x] = make_int2(0, 0);
+    return;
+  }
   if (mine > 0) {
     const long long mine0 = before + incl - mine;
     for (int w = 0; w < kPdWarps; ++w) {
@@ -377,7 +380,6 @@ __global__ void __launch_bounds__(kPdThreads, 1) paged_decode_kernel(const Paged
       const int item = cur.b * H + cur.hh;
       if (starts && ends) {
         w.store_out(p, cur.b, head_of(cur), rows_of(cur), lane);
-        if (lane == 0) p.meta[item] = make_int2(0, 0);
       } else {
         const int e = 2 * warp + (starts ? 1 : 0);
         if (lane == 0) {
@@ -405,6 +407,7 @@ __global__ void __launch_bounds__(kPdThreads, 1) paged_decode_kernel(const Paged
   __syncthreads();
 
   // ---- pieces of one item follow one another in the entries
+  int2 open = make_int2(0, 0);
   for (int e = 0; e < 2 * kPdWarps;) {
     const int item = sm_item[e];
     if (item < 0) {
@@ -417,7 +420,7 @@ __global__ void __launch_bounds__(kPdThreads, 1) paged_decode_kernel(const Paged
     const int rows = min(ROWS, p.group - hb * ROWS);
     const int more = sm_runs[e];
     const bool starts = e & 1;
-    if (tid == 0 && starts) p.meta[item] = make_int2((int)blockIdx.x, more ? more + 1 : 0);
+    if (starts && more) open = make_int2(item, more + 1);
     float* slot = p.part + (long long)(2 * blockIdx.x + (starts ? 1 : 0)) * S::kPiece;
     auto piece = [&](int i) {
       return reinterpret_cast<const float*>(smem + ((i & 1) ? (i >> 1) * S::kRing : kPdWarps * S::kRing +
@@ -450,48 +453,88 @@ __global__ void __launch_bounds__(kPdThreads, 1) paged_decode_kernel(const Paged
     }
     e = end;
   }
+  if (tid == 0) p.meta[blockIdx.x] = open;
 }
 
-// Joins the pieces of every item that several CTAs hold, in the order of the
-// line, and writes zeros for sequences without a visible key. One block per item.
+// Joins the pieces of the items that several CTAs hold, in the order of the
+// line: block (c, r) row r of the one that begins in CTA c, if there is one (a
+// CTA's end cuts one item at most). Its warps take the pieces in turn, then merge.
+// The blocks also write zeros for sequences without a visible key.
 template <typename T, int HD, int ROWS>
-__global__ void __launch_bounds__(HD) paged_join_kernel(const PagedDecodeParams p) {
+__global__ void __launch_bounds__(kPdThreads) paged_join_kernel(const PagedDecodeParams p) {
   using S = DecodeShape<HD, ROWS>;
+  constexpr int V = HD / 32;   // dims per lane
+  __shared__ float sm_acc[kPdWarps][HD], sm_m[kPdWarps], sm_l[kPdWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = lane * V;
+  const int H = p.c.nkv * p.hblocks, r = blockIdx.y;
   pdl_wait();
   pdl_launch_dependents();
-  const int H = p.c.nkv * p.hblocks;
-  const int b = blockIdx.x / H, hh = blockIdx.x - b * H;
-  const int kvh = hh / p.hblocks, hb = hh - kvh * p.hblocks;
-  const int rows = min(ROWS, p.group - hb * ROWS);
-  T* dst = static_cast<T*>(p.out) + b * p.o_b + (long long)(kvh * p.group + hb * ROWS) * p.o_h;
-  const int d = (threadIdx.x % (HD / 2)) * 2;
-  if (seq_len(p.c, b) == 0) {
-    for (int r = threadIdx.x / (HD / 2); r < rows; r += 2) *reinterpret_cast<uint32_t*>(dst + r * p.o_h + d) = 0u;
-    return;
-  }
   const int2 mt = p.meta[blockIdx.x];
-  if (mt.y == 0) return;   // written by the one CTA that holds it
-  for (int r = threadIdx.x / (HD / 2); r < rows; r += 2) {
-    auto row = [&](int i) {
-      return p.part + (long long)(i == 0 ? 2 * mt.x + 1 : 2 * (mt.x + i)) * S::kPiece + r * S::kStride;
-    };
-    float M = -INFINITY;
-#pragma unroll 8
-    for (int i = 0; i < mt.y; ++i) M = fmaxf(M, row(i)[HD]);
-    float L = 0.f, x = 0.f, y = 0.f;
-#pragma unroll 8
-    for (int i = 0; i < mt.y; ++i) {
-      const float* s = row(i);
-      const float2 ml = *reinterpret_cast<const float2*>(s + HD);
-      const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
-      const float2 v = *reinterpret_cast<const float2*>(s + d);
-      L = fmaf(ml.y, f, L);
-      x = fmaf(v.x, f, x);
-      y = fmaf(v.y, f, y);
+  for (int b = blockIdx.x + (int)gridDim.x * warp; b < p.c.B; b += (int)gridDim.x * kPdWarps)
+    if (seq_len(p.c, b) == 0)
+      for (int h = r; h < p.c.nkv * p.group; h += gridDim.y) {
+        T* dst = static_cast<T*>(p.out) + b * p.o_b + h * p.o_h + d;
+        if constexpr (V == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(0, 0);
+        else *reinterpret_cast<uint32_t*>(dst) = 0u;
+      }
+  const int b = mt.x / H, hh = mt.x - b * H, kvh = hh / p.hblocks, hb = hh - kvh * p.hblocks;
+  if (mt.y == 0 || r >= p.group - hb * ROWS) return;
+  constexpr int kAtOnce = 4;
+  float M = -INFINITY, L = 0.f, acc[V] = {};
+  for (int i0 = warp; i0 < mt.y; i0 += kPdWarps * kAtOnce) {
+    float2 ml[kAtOnce];
+    float v[kAtOnce][V];
+#pragma unroll
+    for (int x = 0; x < kAtOnce; ++x) {
+      const int i = i0 + x * kPdWarps;
+      ml[x] = make_float2(-INFINITY, 0.f);
+      if (i < mt.y) {
+        const float* s = p.part + (long long)(i == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + i)) * S::kPiece +
+                         r * S::kStride;
+        ml[x] = *reinterpret_cast<const float2*>(s + HD);
+        if constexpr (V == 4) *reinterpret_cast<float4*>(v[x]) = *reinterpret_cast<const float4*>(s + d);
+        else *reinterpret_cast<float2*>(v[x]) = *reinterpret_cast<const float2*>(s + d);
+      }
     }
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    *reinterpret_cast<uint32_t*>(dst + r * p.o_h + d) = Elem<T>::pack(x * inv, y * inv);
+#pragma unroll
+    for (int x = 0; x < kAtOnce; ++x) {
+      if (ml[x].x == -INFINITY && ml[x].y == 0.f) continue;   // past the end, or no key seen in the piece
+      const float mn = fmaxf(M, ml[x].x);
+      const float f0 = ex2(M - mn), f1 = ex2(ml[x].x - mn);
+      M = mn;
+      L = fmaf(L, f0, ml[x].y * f1);
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[e] = fmaf(acc[e], f0, v[x][e] * f1);
+    }
   }
+#pragma unroll
+  for (int e = 0; e < V; ++e) sm_acc[warp][d + e] = acc[e];
+  if (lane == 0) {
+    sm_m[warp] = M;
+    sm_l[warp] = L;
+  }
+  __syncthreads();
+  if (warp) return;
+  M = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < kPdWarps; ++w) M = fmaxf(M, sm_m[w]);
+  L = 0.f;
+#pragma unroll
+  for (int e = 0; e < V; ++e) acc[e] = 0.f;
+#pragma unroll
+  for (int w = 0; w < kPdWarps; ++w) {
+    const float f = sm_m[w] == -INFINITY ? 0.f : ex2(sm_m[w] - M);   // a warp without pieces
+    L = fmaf(sm_l[w], f, L);
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] = fmaf(sm_acc[w][d + e], f, acc[e]);
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  T* dst = static_cast<T*>(p.out) + b * p.o_b + (long long)(kvh * p.group + hb * ROWS + r) * p.o_h + d;
+  if constexpr (V == 4)
+    *reinterpret_cast<uint2*>(dst) = make_uint2(Elem<T>::pack(acc[0] * inv, acc[1] * inv),
+                                                Elem<T>::pack(acc[2] * inv, acc[3] * inv));
+  else
+    *reinterpret_cast<uint32_t*>(dst) = Elem<T>::pack(acc[0] * inv, acc[1] * inv);
 }
 
 // An item per cluster: its CTAs' warps take the tiles in turn.
@@ -615,7 +658,7 @@ DecodePlan decode_plan(const lw_paged_attention_args* a) {
   d.cluster = 8;
   while (d.cluster > 1 && d.items * d.cluster > d.grid) d.cluster /= 2;
   if (d.items * d.cluster > d.grid || keys > 32ll * lw::kPdTile * d.cluster) d.cluster = 0;
-  d.part_off = ((size_t)d.items * sizeof(int2) + 255) & ~(size_t)255;
+  d.part_off = ((size_t)d.grid * sizeof(int2) + 255) & ~(size_t)255;
   d.bytes = d.cluster ? 0 : d.part_off + (size_t)2 * d.grid * d.rows * (a->cache.head_dim + 8) * sizeof(float);
   return d;
 }
@@ -654,7 +697,8 @@ cudaError_t decode_launch(const lw::PagedDecodeParams& p, const DecodePlan& d, c
   if (e != cudaSuccess) return e;
   e = lw_launch(kern, dim3(d.grid), dim3(lw::kPdThreads), smem, s, pdl, p);
   if (e != cudaSuccess) return e;
-  return lw_launch(lw::paged_join_kernel<T, HD, ROWS>, dim3((unsigned)d.items), dim3(HD), 0, s, true, p);
+  return lw_launch(lw::paged_join_kernel<T, HD, ROWS>, dim3(d.grid, std::min(ROWS, d.group)), dim3(lw::kPdThreads), 0, s,
+                   true, p);
 }
 
 template <typename T>
