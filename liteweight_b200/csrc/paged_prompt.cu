@@ -10,7 +10,7 @@
 // masked keys on the diagonal and at a window's edges). It walks the 128-key
 // tiles that any of its rows sees. Tensor memory holds, for each of the two row
 // tiles, S (128 fp32 columns; P in 16 bits overwrites its first 64) and O
-// (head_dim fp32 columns). The ten warps are specialised:
+// (head_dim fp32 columns). Warps are specialised:
 //   warps 0-3, 4-7  softmax of row tile 0 / 1, one row per thread: read S, mask,
 //                   keep the running maximum and sum in fp32, write P. The
 //                   accumulator is rescaled only when a row's maximum has grown
@@ -22,7 +22,8 @@
 //                   its softmax the tensor cores work on the other.
 // tcgen05.mma instructions of one thread run in the order they are issued, so S of
 // the next keys may overwrite P as soon as the product that reads P is issued,
-// and the barrier of S(j) covers O's update j - 1 too.
+// and the barrier of S(j) covers O's update j - 1 too. P is handed over in two
+// halves, so half of the second product runs beside the other half's exponentials.
 //
 // When the row tiles alone leave SMs idle (few rows, a long cache) the keys are
 // cut into slices as well; each writes (m, sum, fp32 O) to the workspace and a
@@ -46,7 +47,11 @@ namespace lw {
 
 constexpr int kPmRows = 128;                 // rows per tile (UMMA M)
 constexpr int kPmKeys = 128;                 // keys per tile
-constexpr int kPmThreads = 320;
+constexpr int kPmThreads = 384;              // three warpgroups: softmax, softmax, copies and MMA
+// Registers per thread after the split: a softmax row holds 128 scores. The sum
+// is what the block is launched with (168 x 384).
+constexpr int kPmSoftmaxRegs = 224, kPmOtherRegs = 56;
+static_assert(2 * 128 * kPmSoftmaxRegs + 128 * kPmOtherRegs <= 168 * kPmThreads, "registers of the launch");
 constexpr int kPmTmaWarp = 8, kPmMmaWarp = 9;
 constexpr long long kPmWaitNs = 2000000000;
 constexpr float kPmGrow = 8.0f;              // log2 of the largest P
@@ -88,6 +93,25 @@ LW_DEV bool find_row_tile(const PromptParams& p, int slot, int& b, int& i0, int&
   return i0 >= 0 && i0 < n && o >= 0 && (long long)o + n <= p.T;
 }
 
+LW_DEV float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+// Two fp32 operations in one instruction.
+LW_DEV uint64_t as_u64(float2 v) { return *reinterpret_cast<uint64_t*>(&v); }
+LW_DEV float2 as_f2(uint64_t v) { return *reinterpret_cast<float2*>(&v); }
+LW_DEV float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t y;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(as_u64(a)), "l"(as_u64(b)), "l"(as_u64(c)));
+  return as_f2(y);
+}
+LW_DEV float2 add2(float2 a, float2 b) {
+  uint64_t y;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(as_u64(a)), "l"(as_u64(b)));
+  return as_f2(y);
+}
+
 template <int HD>
 struct PromptSmem {
   static constexpr int kTile = kPmKeys * HD * 2;              // a K, V or Q tile
@@ -100,7 +124,8 @@ __global__ void __launch_bounds__(kPmThreads, 1) paged_prompt_kernel(const __gri
   using S = PromptSmem<HD>;
   constexpr int NS = S::kSlots, HALVES = HD / 64, HALF = kPmKeys * 128;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  __shared__ __align__(8) unsigned long long bar_q, bar_full[NS], bar_empty[NS], bar_s[2], bar_p[2], bar_o[2], bar_done;
+  __shared__ __align__(8) unsigned long long bar_q, bar_full[NS], bar_empty[NS], bar_s[2], bar_p[2][2], bar_o[2],
+      bar_done;
   __shared__ uint32_t tmem_s;
   __shared__ volatile int abort_s, odd_s;
   __shared__ volatile uint8_t lost_s[8];   // per key tile (mod 8): its 16-key groups whose page id is outside the pool
@@ -145,7 +170,7 @@ __global__ void __launch_bounds__(kPmThreads, 1) paged_prompt_kernel(const __gri
     }
     for (int g = 0; g < 2; ++g) {
       mbar_init(smem_u32(&bar_s[g]), 1);
-      mbar_init(smem_u32(&bar_p[g]), 4);
+      for (int h = 0; h < 2; ++h) mbar_init(smem_u32(&bar_p[g][h]), 4);
       mbar_init(smem_u32(&bar_o[g]), 1);
     }
     mbar_init(smem_u32(&bar_done), 1);
@@ -174,303 +199,319 @@ __global__ void __launch_bounds__(kPmThreads, 1) paged_prompt_kernel(const __gri
     return __shfl_sync(0xffffffffu, wait(bar, parity) ? 1u : 0u, 0) != 0;
   };
 
-  if (warp == kPmTmaWarp) {
-    // ---- copies. Tile i's K is copy 2i of the ring, its V copy 2i + 1. Lane
-    // (page of the tile, half of the head dim) issues one box each.
-    const int pg = min(p.c.page_size, kPmKeys), npg = kPmKeys / pg;   // slots per box, boxes per tile and half
-    const int my_pg = lane % npg, my_half = lane / npg;
-    const bool mine = my_half < HALVES;
-    auto page_at = [&](int i) {   // page of this lane's part of tile i (no_page: zeros)
-      const int first = key_of(i) + my_pg * pg, end = first + pg - 1;
-      if (!(first <= last && (!windowed || end >= lo0 || first < p.sinks))) return p.no_page;
-      return page_id(p.c, b, first);
-    };
-    int issued = 0;
-    if (nt > 0) {
-      if (lane == 0) {
-        tma_prefetch_map(&p.tm_k);
-        tma_prefetch_map(&p.tm_v);
-        const uint32_t bytes = (uint32_t)(HALVES * 128 * p.group * p.rp);
-        mbar_arrive_expect_tx(smem_u32(&bar_q), bytes * ng);
-        for (int g = 0; g < ng; ++g)
-          for (int h = 0; h < HALVES; ++h)
-            tma_load_3d(base + g * S::kTile + h * HALF, &p.tm_q, h * 64, kvh * p.group, tok0 + g * p.rp,
-                        smem_u32(&bar_q));
-      }
-      int page = page_at(0);
-      bool ok = true;
-      for (int i = 0; i < nt && ok; ++i) {
-        const int key0 = key_of(i);
-        const int next = i + 1 < nt ? page_at(i + 1) : 0;   // asked for a tile ahead
-        // a page id outside the pool: its keys (16-key groups) are hidden, its copy is zeros
-        const uint32_t bad_boxes = __ballot_sync(0xffffffffu, page < 0) & ((1u << npg) - 1u);
+  if (warp >= kPmTmaWarp) {
+    // the third warpgroup gives registers to the other two
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPmOtherRegs));
+    if (warp == kPmTmaWarp) {
+      // ---- copies. Tile i's K is copy 2i of the ring, its V copy 2i + 1. Lane
+      // (page of the tile, half of the head dim) issues one box each.
+      const int pg = min(p.c.page_size, kPmKeys), npg = kPmKeys / pg;   // slots per box, boxes per tile and half
+      const int my_pg = lane % npg, my_half = lane / npg;
+      const bool mine = my_half < HALVES;
+      auto page_at = [&](int i) {   // page of this lane's part of tile i (no_page: zeros)
+        const int first = key_of(i) + my_pg * pg, end = first + pg - 1;
+        if (!(first <= last && (!windowed || end >= lo0 || first < p.sinks))) return p.no_page;
+        return page_id(p.c, b, first);
+      };
+      int issued = 0;
+      if (nt > 0) {
         if (lane == 0) {
-          uint32_t groups = 0;
-          for (int x = 0; x < npg; ++x)
-            if ((bad_boxes >> x) & 1u) groups |= ((1u << (pg / 16)) - 1u) << (x * (pg / 16));
-          lost_s[i & 7] = (uint8_t)groups;
+          tma_prefetch_map(&p.tm_k);
+          tma_prefetch_map(&p.tm_v);
+          const uint32_t bytes = (uint32_t)(HALVES * 128 * p.group * p.rp);
+          mbar_arrive_expect_tx(smem_u32(&bar_q), bytes * ng);
+          for (int g = 0; g < ng; ++g)
+            for (int h = 0; h < HALVES; ++h)
+              tma_load_3d(base + g * S::kTile + h * HALF, &p.tm_q, h * 64, kvh * p.group, tok0 + g * p.rp,
+                          smem_u32(&bar_q));
         }
-        const int w = page < 0 ? p.no_page : page;
-        const int slot = key0 & (p.c.page_size - 1);   // within a page of more than 128 slots
-        for (int kv = 0; kv < 2; ++kv) {
-          const int x = 2 * i + kv, s = x % NS;
-          if (x >= NS && !warp_wait(smem_u32(&bar_empty[s]), ((x / NS) - 1) & 1)) {
-            ok = false;
-            break;
+        int page = page_at(0);
+        bool ok = true;
+        for (int i = 0; i < nt && ok; ++i) {
+          const int key0 = key_of(i);
+          const int next = i + 1 < nt ? page_at(i + 1) : 0;   // asked for a tile ahead
+          // a page id outside the pool: its keys (16-key groups) are hidden, its copy is zeros
+          const uint32_t bad_boxes = __ballot_sync(0xffffffffu, page < 0) & ((1u << npg) - 1u);
+          if (lane == 0) {
+            uint32_t groups = 0;
+            for (int x = 0; x < npg; ++x)
+              if ((bad_boxes >> x) & 1u) groups |= ((1u << (pg / 16)) - 1u) << (x * (pg / 16));
+            lost_s[i & 7] = (uint8_t)groups;
           }
-          if (lane == 0) mbar_arrive_expect_tx(smem_u32(&bar_full[s]), S::kTile);
-          __syncwarp();
-          if (mine)
-            tma_load_4d(base + slot_at(s) + my_half * HALF + my_pg * pg * 128, kv ? &p.tm_v : &p.tm_k, my_half * 64, slot,
-                        kvh, w, smem_u32(&bar_full[s]));
-          __syncwarp();
-          issued = x + 1;
+          const int w = page < 0 ? p.no_page : page;
+          const int slot = key0 & (p.c.page_size - 1);   // within a page of more than 128 slots
+          for (int kv = 0; kv < 2; ++kv) {
+            const int x = 2 * i + kv, s = x % NS;
+            if (x >= NS && !warp_wait(smem_u32(&bar_empty[s]), ((x / NS) - 1) & 1)) {
+              ok = false;
+              break;
+            }
+            if (lane == 0) mbar_arrive_expect_tx(smem_u32(&bar_full[s]), S::kTile);
+            __syncwarp();
+            if (mine)
+              tma_load_4d(base + slot_at(s) + my_half * HALF + my_pg * pg * 128, kv ? &p.tm_v : &p.tm_k, my_half * 64, slot,
+                          kvh, w, smem_u32(&bar_full[s]));
+            __syncwarp();
+            issued = x + 1;
+          }
+          page = next;
         }
-        page = next;
-      }
-      // no copy may land after the CTA has ended (immediate unless a wait gave up)
-      if (lane == 0) {
-        mbar_wait_bounded(smem_u32(&bar_q), 0, kPmWaitNs);
-        for (int x = max(0, issued - NS); x < issued; ++x)
-          mbar_wait_bounded(smem_u32(&bar_full[x % NS]), (x / NS) & 1, kPmWaitNs);
-      }
-      __syncwarp();
-    }
-  } else if (warp == kPmMmaWarp) {
-    // ---- tensor cores
-    const bool leader = elect_one_sync();   // one thread issues everything: commits follow its instructions
-    constexpr uint32_t kFmt = std::is_same<T, __half>::value ? 0u : 1u;
-    constexpr uint32_t kCommon = (1u << 4) | (kFmt << 7) | (kFmt << 10) | ((uint32_t)(kPmRows >> 4) << 24);
-    constexpr uint32_t kDescS = kCommon | ((uint32_t)(kPmKeys >> 3) << 17);              // B = K, K-major
-    constexpr uint32_t kDescO = kCommon | ((uint32_t)(HD >> 3) << 17) | (1u << 16);      // B = V, N-major
-    auto scores = [&](int g, int s) {   // S_g = Q_g K^T
-      const uint64_t a = sw128_desc(base + g * S::kTile), k = sw128_desc(base + slot_at(s));
-#pragma unroll
-      for (int x = 0; x < HD / 16; ++x) {
-        const uint64_t o = (uint64_t)((x / 4) * (HALF >> 4) + (x % 4) * 2);
-        tc_mma_f16(tmem + g * kPmKeys, a + o, k + o, kDescS, x != 0);
-      }
-    };
-    auto values = [&](int g, int s, bool first) {   // O_g += P_g V
-      const uint64_t v = sw128_mn_desc(base + slot_at(s), HALF);
-#pragma unroll
-      for (int x = 0; x < kPmKeys / 16; ++x)
-        tc_mma_f16_ts(tmem + 2 * kPmKeys + g * HD, tmem + g * kPmKeys + 8 * x, v + (uint64_t)(x * (2048 >> 4)), kDescO,
-                      !first || x != 0);
-    };
-    if (nt > 0) {
-      bool ok = warp_wait(smem_u32(&bar_q), 0) && warp_wait(smem_u32(&bar_full[0]), 0);
-      if (ok) {
-        tc_fence_after();
-        if (leader) {
-          for (int g = 0; g < ng; ++g) {
-            scores(g, 0);
-            tc_commit(smem_u32(&bar_s[g]));
-          }
-          tc_commit(smem_u32(&bar_empty[0]));
+        // no copy may land after the CTA has ended (immediate unless a wait gave up)
+        if (lane == 0) {
+          mbar_wait_bounded(smem_u32(&bar_q), 0, kPmWaitNs);
+          for (int x = max(0, issued - NS); x < issued; ++x)
+            mbar_wait_bounded(smem_u32(&bar_full[x % NS]), (x / NS) & 1, kPmWaitNs);
         }
         __syncwarp();
       }
-      for (int i = 0; i < nt && ok; ++i) {
-        const int xv = 2 * i + 1, sv = xv % NS, xk = 2 * i + 2, sk = xk % NS;
-        ok = warp_wait(smem_u32(&bar_full[sv]), (xv / NS) & 1);
-        for (int g = 0; g < ng && ok; ++g) {
-          ok = warp_wait(smem_u32(&bar_p[g]), i & 1);
-          if (ok && g == 0 && i + 1 < nt) ok = warp_wait(smem_u32(&bar_full[sk]), (xk / NS) & 1);
-          if (!ok) break;
+    } else if (warp == kPmMmaWarp) {
+      // ---- tensor cores
+      const bool leader = elect_one_sync();   // one thread issues everything: commits follow its instructions
+      constexpr uint32_t kFmt = std::is_same<T, __half>::value ? 0u : 1u;
+      constexpr uint32_t kCommon = (1u << 4) | (kFmt << 7) | (kFmt << 10) | ((uint32_t)(kPmRows >> 4) << 24);
+      constexpr uint32_t kDescS = kCommon | ((uint32_t)(kPmKeys >> 3) << 17);              // B = K, K-major
+      constexpr uint32_t kDescO = kCommon | ((uint32_t)(HD >> 3) << 17) | (1u << 16);      // B = V, N-major
+      auto scores = [&](int g, int s) {   // S_g = Q_g K^T
+        const uint64_t a = sw128_desc(base + g * S::kTile), k = sw128_desc(base + slot_at(s));
+#pragma unroll
+        for (int x = 0; x < HD / 16; ++x) {
+          const uint64_t o = (uint64_t)((x / 4) * (HALF >> 4) + (x % 4) * 2);
+          tc_mma_f16(tmem + g * kPmKeys, a + o, k + o, kDescS, x != 0);
+        }
+      };
+      auto values = [&](int g, int s, int h, bool first) {   // O_g += P_g V, keys of half h
+        const uint64_t v = sw128_mn_desc(base + slot_at(s), HALF);
+#pragma unroll
+        for (int y = 0; y < kPmKeys / 32; ++y) {
+          const int x = h * (kPmKeys / 32) + y;
+          tc_mma_f16_ts(tmem + 2 * kPmKeys + g * HD, tmem + g * kPmKeys + 8 * x, v + (uint64_t)(x * (2048 >> 4)), kDescO,
+                        !first || x != 0);
+        }
+      };
+      if (nt > 0) {
+        bool ok = warp_wait(smem_u32(&bar_q), 0) && warp_wait(smem_u32(&bar_full[0]), 0);
+        if (ok) {
           tc_fence_after();
           if (leader) {
-            values(g, sv, i == 0);
-            if (g == ng - 1) tc_commit(smem_u32(&bar_empty[sv]));
-            if (i + 1 < nt) {
-              scores(g, sk);
+            for (int g = 0; g < ng; ++g) {
+              scores(g, 0);
               tc_commit(smem_u32(&bar_s[g]));
-              if (g == ng - 1) tc_commit(smem_u32(&bar_empty[sk]));
-            } else {
-              tc_commit(smem_u32(&bar_o[g]));
             }
+            tc_commit(smem_u32(&bar_empty[0]));
           }
           __syncwarp();
         }
+        for (int i = 0; i < nt && ok; ++i) {
+          const int xv = 2 * i + 1, sv = xv % NS, xk = 2 * i + 2, sk = xk % NS;
+          ok = warp_wait(smem_u32(&bar_full[sv]), (xv / NS) & 1);
+          for (int g = 0; g < ng && ok; ++g) {
+            ok = warp_wait(smem_u32(&bar_p[g][0]), i & 1);
+            if (!ok) break;
+            tc_fence_after();
+            if (leader) values(g, sv, 0, i == 0);
+            __syncwarp();
+            ok = warp_wait(smem_u32(&bar_p[g][1]), i & 1);
+            if (ok && g == 0 && i + 1 < nt) ok = warp_wait(smem_u32(&bar_full[sk]), (xk / NS) & 1);
+            if (!ok) break;
+            tc_fence_after();
+            if (leader) {
+              values(g, sv, 1, i == 0);
+              if (g == ng - 1) tc_commit(smem_u32(&bar_empty[sv]));
+              if (i + 1 < nt) {
+                scores(g, sk);
+                tc_commit(smem_u32(&bar_s[g]));
+                if (g == ng - 1) tc_commit(smem_u32(&bar_empty[sk]));
+              } else {
+                tc_commit(smem_u32(&bar_o[g]));
+              }
+            }
+            __syncwarp();
+          }
+        }
+        // tensor memory may not be released under a running instruction
+        if (leader) {
+          tc_commit(smem_u32(&bar_done));
+          mbar_wait_bounded(smem_u32(&bar_done), 0, kPmWaitNs);
+        }
+        __syncwarp();
       }
-      // tensor memory may not be released under a running instruction
-      if (leader) {
-        tc_commit(smem_u32(&bar_done));
-        mbar_wait_bounded(smem_u32(&bar_done), 0, kPmWaitNs);
-      }
-      __syncwarp();
     }
-  } else if (warp / 4 < ng) {
-    // ---- softmax of row tile g, row r
-    const int g = warp >> 2, r = tid & 127;
-    const int npos = min(p.rp, np - g * p.rp);
-    const bool have = r < npos * p.group;
-    const int first_pos = pos0 + g * p.rp, last_pos = min(first_pos + npos, len) - 1;
-    const int pos = have ? min(first_pos + r / p.group, len - 1) : -1;
-    const int lo = windowed ? pos - p.window : -1;   // keys above lo, or below sinks
-    const int sinks = windowed ? p.sinks : 0;
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t ts = tmem + lanes + g * kPmKeys, to = tmem + lanes + 2 * kPmKeys + g * HD;
-    auto sees = [&](int key) { return key <= pos && (key > lo || key < sinks); };
-    float m = -INFINITY, l = 0.f;
-    bool ok = true;
-    for (int i = 0; i < nt; ++i) {
-      if (!(ok = warp_wait(smem_u32(&bar_s[g]), i & 1))) break;
-      tc_fence_after();
-      const int key0 = key_of(i);
-      uint32_t s[4][32];
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPmSoftmaxRegs));
+    if (warp / 4 < ng) {
+      // ---- softmax of row tile g, row r
+      const int g = warp >> 2, r = tid & 127;
+      const int npos = min(p.rp, np - g * p.rp);
+      const bool have = r < npos * p.group;
+      const int first_pos = pos0 + g * p.rp, last_pos = min(first_pos + npos, len) - 1;
+      const int pos = have ? min(first_pos + r / p.group, len - 1) : -1;
+      const int lo = windowed ? pos - p.window : -1;   // keys above lo, or below sinks
+      const int sinks = windowed ? p.sinks : 0;
+      const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+      const uint32_t ts = tmem + lanes + g * kPmKeys, to = tmem + lanes + 2 * kPmKeys + g * HD;
+      auto sees = [&](int key) { return key <= pos && (key > lo || key < sinks); };
+      float m = -INFINITY, l = 0.f;
+      bool ok = true;
+      for (int i = 0; i < nt; ++i) {
+        if (!(ok = warp_wait(smem_u32(&bar_s[g]), i & 1))) break;
+        tc_fence_after();
+        const int key0 = key_of(i);
+        uint32_t s[4][32];
 #pragma unroll
-      for (int x = 0; x < 4; ++x) tmem_ld32(ts + 32 * x, s[x]);
-      tmem_wait_ld();
+        for (int x = 0; x < 4; ++x) tmem_ld32(ts + 32 * x, s[x]);
+        tmem_wait_ld();
 #pragma unroll
-      for (int x = 0; x < 4; ++x) tmem_regs_ready(s[x]);
-      const uint32_t lost = lost_s[i & 7];
-      const bool partial = key0 + kPmKeys - 1 > first_pos || (windowed && key0 <= last_pos - p.window) || lost;
-      if (partial) {
+        for (int x = 0; x < 4; ++x) tmem_regs_ready(s[x]);
+        const uint32_t lost = lost_s[i & 7];
+        const bool partial = key0 + kPmKeys - 1 > first_pos || (windowed && key0 <= last_pos - p.window) || lost;
+        if (partial) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
+          for (int x = 0; x < 4; ++x)
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (!sees(key0 + 32 * x + e) || ((lost >> (2 * x + e / 16)) & 1u)) s[x][e] = __float_as_uint(-INFINITY);
+            for (int e = 0; e < 32; ++e)
+              if (!sees(key0 + 32 * x + e) || ((lost >> (2 * x + e / 16)) & 1u)) s[x][e] = __float_as_uint(-INFINITY);
+        }
+        float mx[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          mx[x] = max3(__uint_as_float(s[x][0]), __uint_as_float(s[x][1]), __uint_as_float(s[x][2]));
+#pragma unroll
+          for (int e = 3; e < 31; e += 2) mx[x] = max3(mx[x], __uint_as_float(s[x][e]), __uint_as_float(s[x][e + 1]));
+          mx[x] = fmaxf(mx[x], __uint_as_float(s[x][31]));
+        }
+        const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+        if (i == 0) {
+          m = mt;
+        } else {
+          const bool grow = mt > m + kPmGrow;
+          if (__any_sync(0xffffffffu, grow)) {
+            // O's update i - 1 is complete (S(i) was issued after it)
+            const float f = !grow ? 1.f : (m == -INFINITY ? 0.f : ex2(m - mt));
+            if (grow) m = mt;
+            l *= f;
+#pragma unroll
+            for (int x = 0; x < HD / 32; ++x) {
+              uint32_t o[32];
+              tmem_ld32(to + 32 * x, o);
+              tmem_wait_ld();
+              tmem_regs_ready(o);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st32(to + 32 * x, o);
+            }
+          }
+        }
+        if (g == 0 && (key0 + kPmKeys - 1 > pos0 || (windowed && key0 <= last - p.window))) {
+          // V's row r of a tile that some row does not see whole
+          const int xv = 2 * i + 1;
+          if (!(ok = warp_wait(smem_u32(&bar_full[xv % NS]), (xv / NS) & 1))) break;
+          uint8_t* row = base_ptr + slot_at(xv % NS) + r * 128;
+          const int key = key0 + r;
+          const bool anyone = key <= last && (!windowed || key >= lo0 || key < p.sinks);
+          for (int c = 0; c < HALVES * 8; ++c) {
+            uint8_t* at = row + (c / 8) * HALF + (((c + r) & 7) << 4);   // the order does not matter: spread over the banks
+            const uint4 v = lds128(at);
+            uint32_t u[4] = {v.x, v.y, v.z, v.w};
+            bool hit = false;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) hit |= has_nonfinite<T>(u[e]);
+            if (hit) {
+              constexpr uint32_t kLo = Elem<T>::kExpMask, kHi = kLo << 16;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                if ((u[e] & kLo) == kLo) u[e] &= 0xFFFF0000u;
+                if ((u[e] & kHi) == kHi) u[e] &= 0x0000FFFFu;
+              }
+              sts128(at, make_uint4(u[0], u[1], u[2], u[3]));
+              if (anyone) odd_s = 1;
+            }
+          }
+          fence_proxy_async_smem();   // before the tensor cores read it
+        }
+        const float sub = m == -INFINITY ? 0.f : m;   // no key seen yet: every weight is 0
+        const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), sub2 = make_float2(-sub, -sub);
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          // weights rounded to T for the second product: half a step each, averaged
+          // over the keys; their sum is that of the unrounded ones
+          uint32_t w[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const int x = 2 * h + e / 16, y = (2 * e) % 32;
+            float2 a = fma2(make_float2(__uint_as_float(s[x][y]), __uint_as_float(s[x][y + 1])), scale2, sub2);
+            a.x = ex2(a.x);
+            a.y = ex2(a.y);
+            sum[e & 1] = add2(sum[e & 1], a);
+            w[e] = Elem<T>::pack(a.x, a.y);
+          }
+          tmem_st32(ts + 32 * h, w);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&bar_p[g][h]));
+        }
+        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       }
-      float mx[4];
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        mx[x] = __uint_as_float(s[x][0]);
-#pragma unroll
-        for (int e = 1; e < 32; ++e) mx[x] = fmaxf(mx[x], __uint_as_float(s[x][e]));
+      // ---- the row's result
+      if (nt > 0 && ok) {
+        ok = warp_wait(smem_u32(&bar_o[g]), 0);
+        tc_fence_after();
       }
-      const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
-      if (i == 0) {
-        m = mt;
-      } else {
-        const bool grow = mt > m + kPmGrow;
-        if (__any_sync(0xffffffffu, grow)) {
-          // O's update i - 1 is complete (S(i) was issued after it)
-          const float f = !grow ? 1.f : (m == -INFINITY ? 0.f : ex2(m - mt));
-          if (grow) m = mt;
-          l *= f;
-#pragma unroll
-          for (int x = 0; x < HD / 32; ++x) {
-            uint32_t o[32];
+      if (ok) {
+        const int tok = tok0 + g * p.rp + (have ? r / p.group : 0), head = kvh * p.group + (have ? r % p.group : 0);
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const bool odd = odd_s;
+        const long long at = ((long long)slice * p.T + tok) * p.nq + head;
+        if (p.slices > 1 && have) p.part_ml[at] = make_float2(nt > 0 ? m : -INFINITY, l);
+#pragma unroll 1
+        for (int x = 0; x < HD / 32; ++x) {
+          uint32_t o[32];
+          if (nt > 0) {
             tmem_ld32(to + 32 * x, o);
             tmem_wait_ld();
             tmem_regs_ready(o);
+          } else {
+            if (p.slices > 1) break;   // nothing of this slice is read
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-            tmem_st32(to + 32 * x, o);
+            for (int e = 0; e < 32; ++e) o[e] = 0u;
           }
-        }
-      }
-      const float sub = m == -INFINITY ? 0.f : m;   // no key seen yet: every weight is 0
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          if (odd && have) {
+            // the values that were cleared and that this row sees
+            for (int i = 0; i < nt; ++i) {
+              const int key0 = key_of(i);
+              if (!(key0 + kPmKeys - 1 > pos0 || (windowed && key0 <= last - p.window))) continue;
+              for (int key = key0; key < key0 + kPmKeys; ++key) {
+                if (!sees(key)) continue;
+                const int page = page_id(p.c, b, key);
+                if (page < 0) continue;
+                const T* v = static_cast<const T*>(p.c.v) + page * p.c.vp + kvh * p.c.vh +
+                             (key & (p.c.page_size - 1)) * p.c.vs + 32 * x;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        // weights rounded to T for the second product: half a step each, averaged
-        // over the keys; their sum is that of the unrounded ones
-        uint32_t w[32];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const int x = 2 * h + e / 16, y = (2 * e) % 32;
-          const float a = ex2(fmaf(__uint_as_float(s[x][y]), p.scale_log2, -sub));
-          const float c = ex2(fmaf(__uint_as_float(s[x][y + 1]), p.scale_log2, -sub));
-          sum[e & 1] += a;
-          sum[2 + (e & 1)] += c;
-          w[e] = Elem<T>::pack(a, c);
-        }
-        tmem_st32(ts + 32 * h, w);
-      }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      if (g == 0 && (key0 + kPmKeys - 1 > pos0 || (windowed && key0 <= last - p.window))) {
-        // V's row r of a tile that some row does not see whole
-        const int xv = 2 * i + 1;
-        if (!(ok = warp_wait(smem_u32(&bar_full[xv % NS]), (xv / NS) & 1))) break;
-        uint8_t* row = base_ptr + slot_at(xv % NS) + r * 128;
-        const int key = key0 + r;
-        const bool anyone = key <= last && (!windowed || key >= lo0 || key < p.sinks);
-        for (int c = 0; c < HALVES * 8; ++c) {
-          uint8_t* at = row + (c / 8) * HALF + (((c + r) & 7) << 4);   // the order does not matter: spread over the banks
-          const uint4 v = lds128(at);
-          uint32_t u[4] = {v.x, v.y, v.z, v.w};
-          bool hit = false;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) hit |= has_nonfinite<T>(u[e]);
-          if (hit) {
-            constexpr uint32_t kLo = Elem<T>::kExpMask, kHi = kLo << 16;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if ((u[e] & kLo) == kLo) u[e] &= 0xFFFF0000u;
-              if ((u[e] & kHi) == kHi) u[e] &= 0x0000FFFFu;
-            }
-            sts128(at, make_uint4(u[0], u[1], u[2], u[3]));
-            if (anyone) odd_s = 1;
-          }
-        }
-        fence_proxy_async_smem();   // before the tensor cores read it
-      }
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&bar_p[g]));
-    }
-    // ---- the row's result
-    if (nt > 0 && ok) {
-      ok = warp_wait(smem_u32(&bar_o[g]), 0);
-      tc_fence_after();
-    }
-    if (ok) {
-      const int tok = tok0 + g * p.rp + (have ? r / p.group : 0), head = kvh * p.group + (have ? r % p.group : 0);
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      const bool odd = odd_s;
-      const long long at = ((long long)slice * p.T + tok) * p.nq + head;
-      if (p.slices > 1 && have) p.part_ml[at] = make_float2(nt > 0 ? m : -INFINITY, l);
-#pragma unroll 1
-      for (int x = 0; x < HD / 32; ++x) {
-        uint32_t o[32];
-        if (nt > 0) {
-          tmem_ld32(to + 32 * x, o);
-          tmem_wait_ld();
-          tmem_regs_ready(o);
-        } else {
-          if (p.slices > 1) break;   // nothing of this slice is read
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0u;
-        }
-        if (odd && have) {
-          // the values that were cleared and that this row sees
-          for (int i = 0; i < nt; ++i) {
-            const int key0 = key_of(i);
-            if (!(key0 + kPmKeys - 1 > pos0 || (windowed && key0 <= last - p.window))) continue;
-            for (int key = key0; key < key0 + kPmKeys; ++key) {
-              if (!sees(key)) continue;
-              const int page = page_id(p.c, b, key);
-              if (page < 0) continue;
-              const T* v = static_cast<const T*>(p.c.v) + page * p.c.vp + kvh * p.c.vh +
-                           (key & (p.c.page_size - 1)) * p.c.vs + 32 * x;
-#pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                const float f = static_cast<float>(v[e]);
-                if (!isfinite(f)) o[e] = __float_as_uint(__uint_as_float(o[e]) + f);
+                for (int e = 0; e < 32; ++e) {
+                  const float f = static_cast<float>(v[e]);
+                  if (!isfinite(f)) o[e] = __float_as_uint(__uint_as_float(o[e]) + f);
+                }
               }
             }
           }
-        }
-        if (!have) continue;
-        if (p.slices > 1) {
-          float4* dst = reinterpret_cast<float4*>(p.part_o + at * HD + 32 * x);
+          if (!have) continue;
+          if (p.slices > 1) {
+            float4* dst = reinterpret_cast<float4*>(p.part_o + at * HD + 32 * x);
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            dst[e] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]),
-                                 __uint_as_float(o[4 * e + 3]));
-        } else {
-          uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + tok * p.o_t + head * p.o_h + 32 * x);
+            for (int e = 0; e < 8; ++e)
+              dst[e] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]),
+                                   __uint_as_float(o[4 * e + 3]));
+          } else {
+            uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + tok * p.o_t + head * p.o_h + 32 * x);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            uint32_t u[4];
+            for (int e = 0; e < 4; ++e) {
+              uint32_t u[4];
 #pragma unroll
-            for (int f = 0; f < 4; ++f)
-              u[f] = Elem<T>::pack(__uint_as_float(o[8 * e + 2 * f]) * inv, __uint_as_float(o[8 * e + 2 * f + 1]) * inv);
-            dst[e] = make_uint4(u[0], u[1], u[2], u[3]);
+              for (int f = 0; f < 4; ++f)
+                u[f] = Elem<T>::pack(__uint_as_float(o[8 * e + 2 * f]) * inv, __uint_as_float(o[8 * e + 2 * f + 1]) * inv);
+              dst[e] = make_uint4(u[0], u[1], u[2], u[3]);
+            }
           }
         }
       }
