@@ -18,6 +18,12 @@ struct Elem<__half> {
   static LW_DEV uint32_t pack(float lo, float hi) { return h2_as_u32(__floats2half2_rn(lo, hi)); }
   static LW_DEV float2 unpack(uint32_t u) { return __half22float2(u32_as_h2(u)); }
   static constexpr uint32_t kExpMask = 0x7C00u;   // all ones: infinity or NaN
+  // a * 0 + c in each half
+  static LW_DEV uint32_t fma0(uint32_t a, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(0u), "r"(c));
+    return d;
+  }
 };
 
 template <>
@@ -30,6 +36,11 @@ struct Elem<__nv_bfloat16> {
     return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
   }
   static constexpr uint32_t kExpMask = 0x7F80u;
+  static LW_DEV uint32_t fma0(uint32_t a, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(0u), "r"(c));
+    return d;
+  }
 };
 
 // Either half of the word is an infinity or a NaN.
@@ -101,9 +112,8 @@ struct PagedView {
   const int* lens;
 };
 
-// Tokens of sequence b the table can address (a longer length is recorded and cut).
-LW_DEV int seq_len(const PagedView& c, int b) {
-  const int n = c.lens[b];
+// Tokens of a sequence of length n that the table can address (a longer length is recorded and cut).
+LW_DEV int cut_len(const PagedView& c, int n) {
   const long long most = (long long)c.table_width << c.page_shift;
   if (n > most) {
     lw_record_error(LW_ERR_BAD_INDEX);
@@ -111,6 +121,7 @@ LW_DEV int seq_len(const PagedView& c, int b) {
   }
   return max(n, 0);
 }
+LW_DEV int seq_len(const PagedView& c, int b) { return cut_len(c, c.lens[b]); }
 
 // Page of token `tok` (0 <= tok < seq_len), or -1 (recorded) for an id outside the pool.
 LW_DEV int page_id(const PagedView& c, int b, int tok) {

@@ -4,13 +4,13 @@
 //
 //   S = scale Q K^T, P = exp2(S log2(e) - m), O = sum P V / sum P
 //
-// on the 5th-generation tensor cores. A CTA (one per SM) takes two tiles of 128
-// rows; a row is a position x a query head of one kv head's group, so K and V
-// are read once for the group and a tile spans only 128 / group positions (few
-// masked keys on the diagonal and at a window's edges). It walks the 128-key
-// tiles that any of its rows sees. Tensor memory holds, for each of the two row
-// tiles, S (128 fp32 columns; P in 16 bits overwrites its first 64) and O
-// (head_dim fp32 columns). Warps are specialised:
+// on the 5th-generation tensor cores. A piece of work is two tiles of 128 rows; a
+// row is a position x a query head of one kv head's group, so K and V are read
+// once for the group and a tile spans only 128 / group positions (few masked
+// keys on the diagonal and at a window's edges). It walks the 128-key tiles that
+// any of its rows sees. Tensor memory holds, for each of the two row tiles, S
+// (128 fp32 columns; P in 16 bits overwrites its first 64) and O (head_dim fp32
+// columns). One CTA per SM; warps are specialised:
 //   warps 0-3, 4-7  softmax of row tile 0 / 1, one row per thread: read S, mask,
 //                   keep the running maximum and sum in fp32, write P. The
 //                   accumulator is rescaled only when a row's maximum has grown
@@ -20,10 +20,14 @@
 //   warp 9          issues tcgen05.mma: S_g = Q_g K^T (both from shared memory),
 //                   O_g += P_g V (P from tensor memory). While one row tile is in
 //                   its softmax the tensor cores work on the other.
+//   warp 10         finds the work: its own block's first, then that of blocks
+//                   not yet launched, which it takes over (cluster launch
+//                   control), so copies and products of the next piece run
+//                   beside the end of this one and SMs share the work evenly.
 // tcgen05.mma instructions of one thread run in the order they are issued, so S of
 // the next keys may overwrite P as soon as the product that reads P is issued,
 // and the barrier of S(j) covers O's update j - 1 too. P is handed over in two
-// halves, so half of the second product runs beside the other half's exponentials.
+// parts, so most of the second product runs beside the last exponentials.
 //
 // When the row tiles alone leave SMs idle (few rows, a long cache) the keys are
 // cut into slices as well; each writes (m, sum, fp32 O) to the workspace and a
@@ -52,9 +56,10 @@ constexpr int kPmThreads = 384;              // three warpgroups: softmax, softm
 // is what the block is launched with (168 x 384).
 constexpr int kPmSoftmaxRegs = 224, kPmOtherRegs = 56;
 static_assert(2 * 128 * kPmSoftmaxRegs + 128 * kPmOtherRegs <= 168 * kPmThreads, "registers of the launch");
-constexpr int kPmTmaWarp = 8, kPmMmaWarp = 9;
+constexpr int kPmTmaWarp = 8, kPmMmaWarp = 9, kPmWorkWarp = 10;
 constexpr long long kPmWaitNs = 2000000000;
 constexpr float kPmGrow = 8.0f;              // log2 of the largest P
+constexpr int kPmPart = 96;                  // keys of P's first part
 
 struct PromptParams {
   CUtensorMap tm_q;   // {head_dim, heads, tokens}, box {64, group, rp}
@@ -74,28 +79,71 @@ struct PromptParams {
   float* part_o;          // [slices][T][nq][head_dim]
 };
 
-// Row tiles of the ragged batch: sequence b owns the slots from off[b] / R + b
-// on (R positions per CTA), at least as many as its rows need (ceil(n / R) <=
-// floor((off + n) / R) - floor(off / R) + 1), so a slot finds its sequence by
-// bisection and the grid needs only T and B. Slots without rows exit.
-LW_DEV bool find_row_tile(const PromptParams& p, int slot, int& b, int& i0, int& n) {
-  const int R = 2 * p.rp;
-  int lo = 0, hi = p.c.B;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (p.off[mid] / R + mid <= slot) lo = mid;
-    else hi = mid;
+// A piece of work: up to 2 * rp positions of one sequence x one kv head's group,
+// against a slice of the key tiles they see.
+struct PromptWork {
+  int valid;           // 0: there is no more
+  int kvh, slice, b;
+  int tok0, np;        // first row of q, positions
+  int pos0, last;      // position of the first, of the last
+  int len;
+  int lo0;             // first key that the window of any row reaches
+  int ns, w0, t0, nt;  // tiles 0 .. ns - 1 and w0 .. are seen; the slice is the nt from the t0-th on
+  LW_DEV int key_of(int i) const { return (t0 + i < ns ? t0 + i : w0 + t0 + i - ns) * kPmKeys; }
+};
+
+// The row tiles of block x of the grid: sequence b owns the blocks from
+// off[b] / R + b on (R positions per block), at least as many as its rows need
+// (ceil(n / R) <= floor((off + n) / R) - floor(off / R) + 1), so a block finds its
+// sequence by bisection and the grid needs only T and B. Some blocks have no rows.
+// A whole warp looks, 32 sequences at a time.
+LW_DEV bool find_work(const PromptParams& p, int blocks, int x, int kvh, int slice, PromptWork& w) {
+  const int R = 2 * p.rp, slot = blocks - 1 - x;   // the longest rows first
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = p.c.B, o, n, len;   // off[lo] / R + lo <= slot, and hi's is past it
+  for (;;) {
+    const int step = (hi - lo + 31) / 32, at = min(lo + lane * step, hi - 1);
+    const int off_at = p.off[at], off_next = p.off[at + 1], len_at = p.c.lens[at];
+    const uint32_t ok = __ballot_sync(0xffffffffu, lo + lane * step < hi && off_at / R + at <= slot);
+    const int last = ok ? 31 - __clz(ok) : 0;   // the offsets do not fall, so these are the first lanes
+    if (step == 1) {
+      lo += last;
+      o = __shfl_sync(0xffffffffu, off_at, last);
+      n = __shfl_sync(0xffffffffu, off_next, last) - o;
+      len = __shfl_sync(0xffffffffu, len_at, last);
+      break;
+    }
+    lo += last * step;
+    hi = min(hi, lo + step);
   }
-  b = lo;
-  const int o = p.off[b];
-  n = p.off[b + 1] - o;
-  i0 = (slot - (o / R + b)) * R;
-  return i0 >= 0 && i0 < n && o >= 0 && (long long)o + n <= p.T;
+  const int i0 = (slot - (o / R + lo)) * R;
+  if (!(i0 >= 0 && i0 < n && o >= 0 && (long long)o + n <= p.T)) return false;
+  w.valid = 1;
+  w.kvh = kvh;
+  w.slice = slice;
+  w.b = lo;
+  w.tok0 = o + i0;
+  w.np = min(R, n - i0);
+  w.len = cut_len(p.c, len);
+  w.pos0 = len - n + i0;   // negative: more rows than tokens
+  if (w.pos0 < 0) lw_record_error(LW_ERR_BAD_INDEX);
+  w.last = min(w.pos0 + w.np, w.len) - 1;
+  w.lo0 = window_start(max(w.pos0, 0), p.window);
+  w.w0 = w.lo0 / kPmKeys;
+  w.ns = p.window > 0 ? min((p.sinks + kPmKeys - 1) / kPmKeys, w.w0) : 0;
+  const int all = w.last < 0 ? 0 : w.ns + w.last / kPmKeys + 1 - w.w0;
+  w.t0 = (int)((long long)all * slice / p.slices);
+  w.nt = (int)((long long)all * (slice + 1) / p.slices) - w.t0;
+  return true;
 }
 
+// Bits 0 .. n - 1 (all of them from n = 32 on, none up to 0).
+LW_DEV uint32_t low_bits(int n) { return n >= 32 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << n) - 1u; }
+
+// The largest of three; NaN if one is.
 LW_DEV float max3(float a, float b, float c) {
   float y;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
 // Two fp32 operations in one instruction.
@@ -112,11 +160,54 @@ LW_DEV float2 add2(float2 a, float2 b) {
   return as_f2(y);
 }
 
+// Zeros in the place of the infinities and NaNs of a row of V (128 bytes in each half).
+template <typename T>
+__device__ __noinline__ void clear_nonfinite(uint8_t* row, int halves, int half_bytes) {
+  for (int h = 0; h < halves; ++h)
+    for (int c = 0; c < 32; ++c) {
+      uint32_t* at = reinterpret_cast<uint32_t*>(row + h * half_bytes) + c;
+      constexpr uint32_t kLo = Elem<T>::kExpMask, kHi = kLo << 16;
+      uint32_t u = *at;
+      if ((u & kLo) == kLo) u &= 0xFFFF0000u;
+      if ((u & kHi) == kHi) u &= 0x0000FFFFu;
+      *at = u;
+    }
+}
+
+// What was cleared and the row sees, added to its accumulator (whole warps).
+template <typename T, int HD>
+__device__ __noinline__ void add_nonfinite(const PromptParams& p, const PromptWork& w, int pos, int lo, int sinks,
+                                           uint32_t to) {
+  for (int x = 0; x < HD / 8; ++x) {
+    uint32_t o[8];
+    tmem_ld8(to + 8 * x, o);
+    for (int i = 0; i < w.nt; ++i) {
+      const int key0 = w.key_of(i);
+      if (!(key0 + kPmKeys - 1 > w.pos0 || (p.window > 0 && key0 <= w.last - p.window))) continue;
+      for (int key = key0; key < key0 + kPmKeys; ++key) {
+        if (!(key <= pos && (key > lo || key < sinks))) continue;
+        const int page = page_id(p.c, w.b, key);
+        if (page < 0) continue;
+        const T* v = static_cast<const T*>(p.c.v) + page * p.c.vp + w.kvh * p.c.vh + (key & (p.c.page_size - 1)) * p.c.vs +
+                     8 * x;
+        for (int e = 0; e < 8; ++e) {
+          const float f = static_cast<float>(v[e]);
+          if (!isfinite(f)) o[e] = __float_as_uint(__uint_as_float(o[e]) + f);
+        }
+      }
+    }
+    __syncwarp();
+    tmem_st8(to + 8 * x, o);
+  }
+  tmem_wait_st();
+}
+
 template <int HD>
 struct PromptSmem {
   static constexpr int kTile = kPmKeys * HD * 2;              // a K, V or Q tile
-  static constexpr int kSlots = HD == 128 ? 5 : 8;            // K and V tiles in the ring
-  static constexpr int kBytes = 1024 + (2 + kSlots) * kTile;
+  static constexpr int kSlots = HD == 128 ? 4 : 8;            // K and V tiles in the ring
+  static constexpr int kStage = 32 * 128;                     // a softmax warp's 32 rows, 128 bytes at a time, on their way out
+  static constexpr int kBytes = 1024 + (2 + kSlots) * kTile + 8 * kStage;
 };
 
 template <typename T, int HD>
@@ -124,46 +215,22 @@ __global__ void __launch_bounds__(kPmThreads, 1) paged_prompt_kernel(const __gri
   using S = PromptSmem<HD>;
   constexpr int NS = S::kSlots, HALVES = HD / 64, HALF = kPmKeys * 128;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  __shared__ __align__(8) unsigned long long bar_q, bar_full[NS], bar_empty[NS], bar_s[2], bar_p[2][2], bar_o[2],
-      bar_done;
+  __shared__ __align__(16) uint4 clc_s;
+  __shared__ __align__(8) unsigned long long bar_q, bar_qfree, bar_full[NS], bar_empty[NS], bar_s[2], bar_p[2][2], bar_o[2],
+      bar_work, bar_taken, bar_clc, bar_done;
+  __shared__ PromptWork work_s;
   __shared__ uint32_t tmem_s;
-  __shared__ volatile int abort_s, odd_s;
-  __shared__ volatile uint8_t lost_s[8];   // per key tile (mod 8): its 16-key groups whose page id is outside the pool
+  __shared__ volatile int abort_s, odd_s[4];   // odd_s[piece mod 4]: a value was cleared that rows see
+  __shared__ volatile uint8_t lost_s[8];       // key tile mod 8: its 16-key groups whose page id is outside the pool
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int kvh = blockIdx.y, slice = blockIdx.z;
-  pdl_wait();
-  pdl_launch_dependents();
-  if (p.zero_tail && slice == 0) {
-    for (int r = max(0, p.off[p.c.B]) + blockIdx.x; r < p.T; r += gridDim.x)
-      for (int i = tid; i < p.group * (HD / 8); i += kPmThreads)
-        *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + r * p.o_t + (kvh * p.group + i / (HD / 8)) * p.o_h +
-                                  (i % (HD / 8)) * 8) = make_uint4(0, 0, 0, 0);
-  }
-  int b, i0, n;
-  if (!find_row_tile(p, gridDim.x - 1 - blockIdx.x, b, i0, n)) return;   // the longest rows first
-  const int tok0 = p.off[b] + i0;
-  const int np = min(2 * p.rp, n - i0);              // positions of this CTA
-  const int ng = np > p.rp ? 2 : 1;                  // row tiles
-  const int len = seq_len(p.c, b);
-  const int pos0 = p.c.lens[b] - n + i0;             // the first position (negative: more rows than tokens)
-  const int last = min(pos0 + np, len) - 1;          // the last one
-  if (pos0 < 0 && tid == 0) lw_record_error(LW_ERR_BAD_INDEX);
-  const bool windowed = p.window > 0;
-  const int lo0 = window_start(max(pos0, 0), p.window);   // the first key the window of any row reaches
-  const int w0 = lo0 / kPmKeys;
-  const int ns = windowed ? min((p.sinks + kPmKeys - 1) / kPmKeys, w0) : 0;   // tiles of first keys before it
-  const int nt_all = last < 0 ? 0 : ns + last / kPmKeys + 1 - w0;
-  const int t0 = (int)((long long)nt_all * slice / p.slices);
-  const int nt = (int)((long long)nt_all * (slice + 1) / p.slices) - t0;   // this slice's tiles
-  auto key_of = [&](int i) { return (t0 + i < ns ? t0 + i : w0 + t0 + i - ns) * kPmKeys; };
-
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* base_ptr = smem_raw + (base - smem_u32(smem_raw));
   auto slot_at = [&](int s) { return (uint32_t)(2 + s) * S::kTile; };
 
   if (tid == 0) {
     mbar_init(smem_u32(&bar_q), 1);
+    mbar_init(smem_u32(&bar_qfree), 1);
     for (int s = 0; s < NS; ++s) {
       mbar_init(smem_u32(&bar_full[s]), 1);
       mbar_init(smem_u32(&bar_empty[s]), 1);
@@ -173,9 +240,12 @@ __global__ void __launch_bounds__(kPmThreads, 1) paged_prompt_kernel(const __gri
       for (int h = 0; h < 2; ++h) mbar_init(smem_u32(&bar_p[g][h]), 4);
       mbar_init(smem_u32(&bar_o[g]), 1);
     }
+    mbar_init(smem_u32(&bar_work), 1);
+    mbar_init(smem_u32(&bar_taken), 10);   // the softmax, copy and MMA warps
+    mbar_init(smem_u32(&bar_clc), 1);
     mbar_init(smem_u32(&bar_done), 1);
     abort_s = 0;
-    odd_s = 0;
+    for (int i = 0; i < 4; ++i) odd_s[i] = 0;
     fence_mbar_init();
   }
   if (warp == kPmMmaWarp) {
@@ -186,6 +256,8 @@ __global__ void __launch_bounds__(kPmThreads, 1) paged_prompt_kernel(const __gri
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_s;
+  pdl_wait();
+  pdl_launch_dependents();
 
   // Bounded waits: the first to give up makes the others stop at their next one.
   auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
@@ -198,72 +270,90 @@ __global__ void __launch_bounds__(kPmThreads, 1) paged_prompt_kernel(const __gri
   auto warp_wait = [&](uint32_t bar, uint32_t parity) -> bool {
     return __shfl_sync(0xffffffffu, wait(bar, parity) ? 1u : 0u, 0) != 0;
   };
+  // The warp's copy of piece `it` (false: no more, or a wait gave up).
+  auto take = [&](int it, PromptWork& w) -> bool {
+    if (!warp_wait(smem_u32(&bar_work), it & 1)) return false;
+    w = work_s;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&bar_taken));
+    return w.valid != 0;
+  };
+  const bool windowed = p.window > 0;
 
   if (warp >= kPmTmaWarp) {
     // the third warpgroup gives registers to the other two
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPmOtherRegs));
     if (warp == kPmTmaWarp) {
-      // ---- copies. Tile i's K is copy 2i of the ring, its V copy 2i + 1. Lane
-      // (page of the tile, half of the head dim) issues one box each.
+      // ---- copies. Tile i's K is copy 2i of the ring, its V copy 2i + 1 (i
+      // counts through all pieces). Lane (page of the tile, half of the head
+      // dim) issues one box each.
       const int pg = min(p.c.page_size, kPmKeys), npg = kPmKeys / pg;   // slots per box, boxes per tile and half
       const int my_pg = lane % npg, my_half = lane / npg;
       const bool mine = my_half < HALVES;
-      auto page_at = [&](int i) {   // page of this lane's part of tile i (no_page: zeros)
-        const int first = key_of(i) + my_pg * pg, end = first + pg - 1;
-        if (!(first <= last && (!windowed || end >= lo0 || first < p.sinks))) return p.no_page;
-        return page_id(p.c, b, first);
-      };
-      int issued = 0;
-      if (nt > 0) {
-        if (lane == 0) {
-          tma_prefetch_map(&p.tm_k);
-          tma_prefetch_map(&p.tm_v);
-          const uint32_t bytes = (uint32_t)(HALVES * 128 * p.group * p.rp);
-          mbar_arrive_expect_tx(smem_u32(&bar_q), bytes * ng);
-          for (int g = 0; g < ng; ++g)
-            for (int h = 0; h < HALVES; ++h)
-              tma_load_3d(base + g * S::kTile + h * HALF, &p.tm_q, h * 64, kvh * p.group, tok0 + g * p.rp,
-                          smem_u32(&bar_q));
-        }
-        int page = page_at(0);
-        bool ok = true;
-        for (int i = 0; i < nt && ok; ++i) {
-          const int key0 = key_of(i);
-          const int next = i + 1 < nt ? page_at(i + 1) : 0;   // asked for a tile ahead
+      if (lane == 0) {
+        tma_prefetch_map(&p.tm_q);
+        tma_prefetch_map(&p.tm_k);
+        tma_prefetch_map(&p.tm_v);
+      }
+      int x = 0, s = 0, nq = 0;      // copies issued, the next one's slot, Q loads issued
+      uint32_t phase = 1;            // of the slots' emptiness (the first pass over the ring does not wait)
+      bool ok = true;
+      PromptWork w;
+      for (int it = 0; ok && take(it, w); ++it) {
+        auto page_at = [&](int i) {   // page of this lane's part of tile i (no_page: zeros)
+          const int first = w.key_of(i) + my_pg * pg, end = first + pg - 1;
+          if (!(first <= w.last && (!windowed || end >= w.lo0 || first < p.sinks))) return p.no_page;
+          return page_id(p.c, w.b, first);
+        };
+        int page = w.nt > 0 ? page_at(0) : 0;
+        for (int i = 0; i < w.nt && ok; ++i) {
+          const int key0 = w.key_of(i);
+          const int next = i + 1 < w.nt ? page_at(i + 1) : 0;   // asked for a tile ahead
           // a page id outside the pool: its keys (16-key groups) are hidden, its copy is zeros
           const uint32_t bad_boxes = __ballot_sync(0xffffffffu, page < 0) & ((1u << npg) - 1u);
           if (lane == 0) {
             uint32_t groups = 0;
-            for (int x = 0; x < npg; ++x)
-              if ((bad_boxes >> x) & 1u) groups |= ((1u << (pg / 16)) - 1u) << (x * (pg / 16));
-            lost_s[i & 7] = (uint8_t)groups;
+            for (int y = 0; y < npg; ++y)
+              if ((bad_boxes >> y) & 1u) groups |= ((1u << (pg / 16)) - 1u) << (y * (pg / 16));
+            lost_s[(x >> 1) & 7] = (uint8_t)groups;
           }
-          const int w = page < 0 ? p.no_page : page;
+          const int from = page < 0 ? p.no_page : page;
           const int slot = key0 & (p.c.page_size - 1);   // within a page of more than 128 slots
           for (int kv = 0; kv < 2; ++kv) {
-            const int x = 2 * i + kv, s = x % NS;
-            if (x >= NS && !warp_wait(smem_u32(&bar_empty[s]), ((x / NS) - 1) & 1)) {
-              ok = false;
-              break;
-            }
-            if (lane == 0) mbar_arrive_expect_tx(smem_u32(&bar_full[s]), S::kTile);
+            if (!(ok = warp_wait(smem_u32(&bar_empty[s]), phase))) break;
+            const uint32_t bar = smem_u32(&bar_full[s]);
+            if (lane == 0) mbar_arrive_expect_tx(bar, S::kTile);
             __syncwarp();
             if (mine)
               tma_load_4d(base + slot_at(s) + my_half * HALF + my_pg * pg * 128, kv ? &p.tm_v : &p.tm_k, my_half * 64, slot,
-                          kvh, w, smem_u32(&bar_full[s]));
+                          w.kvh, from, bar);
             __syncwarp();
-            issued = x + 1;
+            ++x;
+            if (++s == NS) s = 0, phase ^= 1u;
+            if (kv == 0 && i == 0) {   // Q once the last scores of the piece before are done
+              if (nq > 0 && !(ok = warp_wait(smem_u32(&bar_qfree), (nq - 1) & 1))) break;
+              if (lane == 0) {
+                const int ng = w.np > p.rp ? 2 : 1;
+                mbar_arrive_expect_tx(smem_u32(&bar_q), (uint32_t)(HALVES * 128 * p.group * p.rp) * ng);
+                for (int g = 0; g < ng; ++g)
+                  for (int h = 0; h < HALVES; ++h)
+                    tma_load_3d(base + g * S::kTile + h * HALF, &p.tm_q, h * 64, w.kvh * p.group, w.tok0 + g * p.rp,
+                                smem_u32(&bar_q));
+              }
+              __syncwarp();
+              ++nq;
+            }
           }
           page = next;
         }
-        // no copy may land after the CTA has ended (immediate unless a wait gave up)
-        if (lane == 0) {
-          mbar_wait_bounded(smem_u32(&bar_q), 0, kPmWaitNs);
-          for (int x = max(0, issued - NS); x < issued; ++x)
-            mbar_wait_bounded(smem_u32(&bar_full[x % NS]), (x / NS) & 1, kPmWaitNs);
-        }
-        __syncwarp();
       }
+      // no copy may land after the CTA has ended (immediate unless a wait gave up)
+      if (lane == 0) {
+        if (nq > 0) mbar_wait_bounded(smem_u32(&bar_q), (nq - 1) & 1, kPmWaitNs);
+        for (int y = max(0, x - NS); y < x; ++y)
+          mbar_wait_bounded(smem_u32(&bar_full[y % NS]), (y / NS) & 1, kPmWaitNs);
+      }
+      __syncwarp();
     } else if (warp == kPmMmaWarp) {
       // ---- tensor cores
       const bool leader = elect_one_sync();   // one thread issues everything: commits follow its instructions
@@ -279,97 +369,169 @@ __global__ void __launch_bounds__(kPmThreads, 1) paged_prompt_kernel(const __gri
           tc_mma_f16(tmem + g * kPmKeys, a + o, k + o, kDescS, x != 0);
         }
       };
-      auto values = [&](int g, int s, int h, bool first) {   // O_g += P_g V, keys of half h
+      auto values = [&](int g, int s, int x0, int x1, bool first) {   // O_g += P_g V, keys 16 x0 .. 16 x1 - 1
         const uint64_t v = sw128_mn_desc(base + slot_at(s), HALF);
 #pragma unroll
-        for (int y = 0; y < kPmKeys / 32; ++y) {
-          const int x = h * (kPmKeys / 32) + y;
+        for (int x = x0; x < x1; ++x)
           tc_mma_f16_ts(tmem + 2 * kPmKeys + g * HD, tmem + g * kPmKeys + 8 * x, v + (uint64_t)(x * (2048 >> 4)), kDescO,
                         !first || x != 0);
-        }
       };
-      if (nt > 0) {
-        bool ok = warp_wait(smem_u32(&bar_q), 0) && warp_wait(smem_u32(&bar_full[0]), 0);
-        if (ok) {
-          tc_fence_after();
-          if (leader) {
-            for (int g = 0; g < ng; ++g) {
-              scores(g, 0);
-              tc_commit(smem_u32(&bar_s[g]));
-            }
-            tc_commit(smem_u32(&bar_empty[0]));
+      int s = 0, nq = 0, np[2] = {0, 0};   // ring slot, Q loads awaited, P tiles of each row tile awaited
+      uint32_t phase = 0;
+      auto step = [&] {
+        if (++s == NS) s = 0, phase ^= 1u;
+      };
+      bool ok = true;
+      PromptWork w;
+      for (int it = 0; ok && take(it, w); ++it) {
+        if (w.nt == 0) continue;
+        const int ng = w.np > p.rp ? 2 : 1;
+        ok = warp_wait(smem_u32(&bar_full[s]), phase) && warp_wait(smem_u32(&bar_q), nq++ & 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (leader) {
+          for (int g = 0; g < ng; ++g) {
+            scores(g, s);
+            tc_commit(smem_u32(&bar_s[g]));
           }
-          __syncwarp();
+          tc_commit(smem_u32(&bar_empty[s]));
+          if (w.nt == 1) tc_commit(smem_u32(&bar_qfree));
         }
-        for (int i = 0; i < nt && ok; ++i) {
-          const int xv = 2 * i + 1, sv = xv % NS, xk = 2 * i + 2, sk = xk % NS;
-          ok = warp_wait(smem_u32(&bar_full[sv]), (xv / NS) & 1);
-          for (int g = 0; g < ng && ok; ++g) {
-            ok = warp_wait(smem_u32(&bar_p[g][0]), i & 1);
-            if (!ok) break;
+        __syncwarp();
+        step();
+        for (int i = 0; i < w.nt && ok; ++i) {
+          const int sv = s;
+          if (!(ok = warp_wait(smem_u32(&bar_full[sv]), phase))) break;
+          step();   // at the next tile's K
+          for (int g = 0; g < ng; ++g) {
+            const uint32_t par = np[g]++ & 1;
+            if (!(ok = warp_wait(smem_u32(&bar_p[g][0]), par))) break;
             tc_fence_after();
-            if (leader) values(g, sv, 0, i == 0);
+            if (leader) values(g, sv, 0, kPmPart / 16, i == 0);
             __syncwarp();
-            ok = warp_wait(smem_u32(&bar_p[g][1]), i & 1);
-            if (ok && g == 0 && i + 1 < nt) ok = warp_wait(smem_u32(&bar_full[sk]), (xk / NS) & 1);
+            ok = warp_wait(smem_u32(&bar_p[g][1]), par);
+            if (ok && g == 0 && i + 1 < w.nt) ok = warp_wait(smem_u32(&bar_full[s]), phase);
             if (!ok) break;
             tc_fence_after();
             if (leader) {
-              values(g, sv, 1, i == 0);
+              values(g, sv, kPmPart / 16, kPmKeys / 16, i == 0);
               if (g == ng - 1) tc_commit(smem_u32(&bar_empty[sv]));
-              if (i + 1 < nt) {
-                scores(g, sk);
+              if (i + 1 < w.nt) {
+                scores(g, s);
                 tc_commit(smem_u32(&bar_s[g]));
-                if (g == ng - 1) tc_commit(smem_u32(&bar_empty[sk]));
+                if (g == ng - 1) {
+                  tc_commit(smem_u32(&bar_empty[s]));
+                  if (i + 2 == w.nt) tc_commit(smem_u32(&bar_qfree));
+                }
               } else {
                 tc_commit(smem_u32(&bar_o[g]));
               }
             }
             __syncwarp();
           }
+          if (ok && i + 1 < w.nt) step();
         }
-        // tensor memory may not be released under a running instruction
-        if (leader) {
-          tc_commit(smem_u32(&bar_done));
-          mbar_wait_bounded(smem_u32(&bar_done), 0, kPmWaitNs);
+      }
+      // tensor memory may not be released under a running instruction
+      if (leader) {
+        tc_commit(smem_u32(&bar_done));
+        mbar_wait_bounded(smem_u32(&bar_done), 0, kPmWaitNs);
+      }
+      __syncwarp();
+    } else if (warp == kPmWorkWarp) {
+      // ---- work: publish a piece, and when every warp has taken it, ask for another
+      int x = blockIdx.x, y = blockIdx.y, z = blockIdx.z, it = 0;
+      uint32_t asked = 0;
+      bool more = true;
+      PromptWork w;
+      auto publish = [&]() -> bool {
+        if (lane == 0) {
+          work_s = w;
+          mbar_arrive(smem_u32(&bar_work));
         }
         __syncwarp();
+        // most of a piece's time: asleep, not polling beside the softmax warps
+        const uint32_t bar = smem_u32(&bar_taken), parity = it++ & 1;
+        const unsigned long long t0 = globaltimer_ns();
+        bool ok = true;
+        while (ok && !mbar_try_wait_sleep(bar, parity, 20000)) {
+          if (abort_s || (long long)(globaltimer_ns() - t0) > kPmWaitNs) {
+            lw_record_error(LW_ERR_TIMEOUT);
+            abort_s = 1;
+            ok = false;
+          }
+        }
+        return __shfl_sync(0xffffffffu, ok ? 1u : 0u, 0) != 0;
+      };
+      while (more) {
+        const int bx = x, by = y, bz = z;
+        if (find_work(p, gridDim.x, x, y, z, w) && !publish()) break;
+        if (lane == 0) {
+          fence_proxy_async_smem();   // the answer before has been read
+          mbar_arrive_expect_tx(smem_u32(&bar_clc), 16);
+          clc_try_cancel(smem_u32(&clc_s), smem_u32(&bar_clc));
+        }
+        __syncwarp();
+        if (!warp_wait(smem_u32(&bar_clc), asked++ & 1)) break;
+        more = clc_answer(smem_u32(&clc_s), x, y, z);
+        __syncwarp();
+        if (p.zero_tail && bz == 0) {   // rows of no sequence
+          for (int r = max(0, p.off[p.c.B]) + bx; r < p.T; r += gridDim.x)
+            for (int i = lane; i < p.group * (HD / 8); i += 32)
+              *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + r * p.o_t + (by * p.group + i / (HD / 8)) * p.o_h +
+                                        (i % (HD / 8)) * 8) = make_uint4(0, 0, 0, 0);
+        }
       }
+      w.valid = 0;
+      if (!more) publish();
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPmSoftmaxRegs));
-    if (warp / 4 < ng) {
-      // ---- softmax of row tile g, row r
-      const int g = warp >> 2, r = tid & 127;
-      const int npos = min(p.rp, np - g * p.rp);
+    // ---- softmax of row tile g, row r
+    const int g = warp >> 2, r = tid & 127, r_pos = r / p.group, r_head = r - r_pos * p.group;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + lanes + g * kPmKeys, to = tmem + lanes + 2 * kPmKeys + g * HD;
+    uint8_t* stage = base_ptr + slot_at(NS) + warp * S::kStage;
+    int tiles = 0, ns = 0, no = 0;   // key tiles of all pieces, S tiles and O tiles of this row tile
+    bool ok = true;
+    PromptWork w;
+    for (int it = 0; ok && take(it, w); ++it) {
+      if (tid == 0) odd_s[(it + 2) & 3] = 0;
+      if (g == 1 && w.np <= p.rp) {   // no second row tile
+        tiles += w.nt;
+        continue;
+      }
+      const int npos = min(p.rp, w.np - g * p.rp);
       const bool have = r < npos * p.group;
-      const int first_pos = pos0 + g * p.rp, last_pos = min(first_pos + npos, len) - 1;
-      const int pos = have ? min(first_pos + r / p.group, len - 1) : -1;
+      const int first_pos = w.pos0 + g * p.rp, last_pos = min(first_pos + npos, w.len) - 1;
+      const int pos = have ? min(first_pos + r_pos, w.len - 1) : -1;
       const int lo = windowed ? pos - p.window : -1;   // keys above lo, or below sinks
       const int sinks = windowed ? p.sinks : 0;
-      const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-      const uint32_t ts = tmem + lanes + g * kPmKeys, to = tmem + lanes + 2 * kPmKeys + g * HD;
-      auto sees = [&](int key) { return key <= pos && (key > lo || key < sinks); };
       float m = -INFINITY, l = 0.f;
-      bool ok = true;
-      for (int i = 0; i < nt; ++i) {
-        if (!(ok = warp_wait(smem_u32(&bar_s[g]), i & 1))) break;
+      // key tiles that a row of this row tile / of the piece does not see whole
+      const int mask_hi = first_pos - (kPmKeys - 1), mask_lo = windowed ? last_pos - p.window : -1;
+      const int cut_hi = w.pos0 - (kPmKeys - 1), cut_lo = windowed ? w.last - p.window : -1;
+      int key0 = w.key_of(0);
+      for (int i = 0; i < w.nt; ++i, ++tiles, key0 = w.t0 + i == w.ns ? w.w0 * kPmKeys : key0 + kPmKeys) {
+        if (!(ok = warp_wait(smem_u32(&bar_s[g]), ns++ & 1))) break;
         tc_fence_after();
-        const int key0 = key_of(i);
         uint32_t s[4][32];
 #pragma unroll
         for (int x = 0; x < 4; ++x) tmem_ld32(ts + 32 * x, s[x]);
         tmem_wait_ld();
 #pragma unroll
         for (int x = 0; x < 4; ++x) tmem_regs_ready(s[x]);
-        const uint32_t lost = lost_s[i & 7];
-        const bool partial = key0 + kPmKeys - 1 > first_pos || (windowed && key0 <= last_pos - p.window) || lost;
-        if (partial) {
+        const uint32_t lost = lost_s[tiles & 7];
+        if (key0 > mask_hi || key0 <= mask_lo || lost) {
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
+          for (int x = 0; x < 4; ++x) {
+            // bit e: the row sees key k0 + e
+            const int k0 = key0 + 32 * x;
+            const uint32_t gone = ((lost >> (2 * x)) & 1u ? 0xFFFFu : 0u) | ((lost >> (2 * x)) & 2u ? 0xFFFF0000u : 0u);
+            const uint32_t seen = low_bits(pos + 1 - k0) & (~low_bits(lo + 1 - k0) | low_bits(sinks - k0)) & ~gone;
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!sees(key0 + 32 * x + e) || ((lost >> (2 * x + e / 16)) & 1u)) s[x][e] = __float_as_uint(-INFINITY);
+            for (int e = 0; e < 32; ++e) s[x][e] = (seen >> e) & 1u ? s[x][e] : 0xFF800000u;   // -infinity
+          }
         }
         float mx[4];
 #pragma unroll
@@ -377,13 +539,14 @@ __global__ void __launch_bounds__(kPmThreads, 1) paged_prompt_kernel(const __gri
           mx[x] = max3(__uint_as_float(s[x][0]), __uint_as_float(s[x][1]), __uint_as_float(s[x][2]));
 #pragma unroll
           for (int e = 3; e < 31; e += 2) mx[x] = max3(mx[x], __uint_as_float(s[x][e]), __uint_as_float(s[x][e + 1]));
-          mx[x] = fmaxf(mx[x], __uint_as_float(s[x][31]));
+          mx[x] = max3(mx[x], mx[x], __uint_as_float(s[x][31]));
         }
-        const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+        // a NaN among the row's scores makes its maximum, and so all of the row, NaN
+        const float mt = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * p.scale_log2;
         if (i == 0) {
-          m = mt;
+          m = have ? mt : 0.f;   // a row that is none holds anything
         } else {
-          const bool grow = mt > m + kPmGrow;
+          const bool grow = have && !(mt <= m + kPmGrow);
           if (__any_sync(0xffffffffu, grow)) {
             // O's update i - 1 is complete (S(i) was issued after it)
             const float f = !grow ? 1.f : (m == -INFINITY ? 0.f : ex2(m - mt));
@@ -401,118 +564,124 @@ __global__ void __launch_bounds__(kPmThreads, 1) paged_prompt_kernel(const __gri
             }
           }
         }
-        if (g == 0 && (key0 + kPmKeys - 1 > pos0 || (windowed && key0 <= last - p.window))) {
-          // V's row r of a tile that some row does not see whole
-          const int xv = 2 * i + 1;
+        if (g == 0 && (key0 > cut_hi || key0 <= cut_lo)) {
+          // row r of V
+          const int xv = 2 * tiles + 1;
           if (!(ok = warp_wait(smem_u32(&bar_full[xv % NS]), (xv / NS) & 1))) break;
-          uint8_t* row = base_ptr + slot_at(xv % NS) + r * 128;
-          const int key = key0 + r;
-          const bool anyone = key <= last && (!windowed || key >= lo0 || key < p.sinks);
+          const uint8_t* row = base_ptr + slot_at(xv % NS) + r * 128;
+          uint32_t any = 0u;   // NaN in either half once an infinity or a NaN has passed: 0 * it
+#pragma unroll
           for (int c = 0; c < HALVES * 8; ++c) {
-            uint8_t* at = row + (c / 8) * HALF + (((c + r) & 7) << 4);   // the order does not matter: spread over the banks
-            const uint4 v = lds128(at);
-            uint32_t u[4] = {v.x, v.y, v.z, v.w};
-            bool hit = false;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) hit |= has_nonfinite<T>(u[e]);
-            if (hit) {
-              constexpr uint32_t kLo = Elem<T>::kExpMask, kHi = kLo << 16;
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                if ((u[e] & kLo) == kLo) u[e] &= 0xFFFF0000u;
-                if ((u[e] & kHi) == kHi) u[e] &= 0x0000FFFFu;
-              }
-              sts128(at, make_uint4(u[0], u[1], u[2], u[3]));
-              if (anyone) odd_s = 1;
-            }
+            const uint4 v = lds128(row + (c / 8) * HALF + (((c + r) & 7) << 4));   // in any order: spread over the banks
+            any = Elem<T>::fma0(v.x, Elem<T>::fma0(v.y, Elem<T>::fma0(v.z, Elem<T>::fma0(v.w, any))));
+          }
+          if (has_nonfinite<T>(any)) {
+            const int key = key0 + r;
+            clear_nonfinite<T>(base_ptr + slot_at(xv % NS) + r * 128, HALVES, HALF);
+            if (key <= w.last && (!windowed || key >= w.lo0 || key < p.sinks)) odd_s[it & 3] = 1;
           }
           fence_proxy_async_smem();   // before the tensor cores read it
         }
         const float sub = m == -INFINITY ? 0.f : m;   // no key seen yet: every weight is 0
         const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), sub2 = make_float2(-sub, -sub);
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        // weights rounded to T for the second product: half a step each, averaged
+        // over the keys; their sum is that of the unrounded ones
+        auto weights = [&](int e) {
+          const int x = e / 16, y = (2 * e) % 32;
+          float2 a = fma2(make_float2(__uint_as_float(s[x][y]), __uint_as_float(s[x][y + 1])), scale2, sub2);
+          a.x = ex2(a.x);
+          a.y = ex2(a.y);
+          sum[e & 1] = add2(sum[e & 1], a);
+          return Elem<T>::pack(a.x, a.y);
+        };
+        static_assert(kPmPart == 96, "the stores below");
+        {
+          uint32_t u[32];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          // weights rounded to T for the second product: half a step each, averaged
-          // over the keys; their sum is that of the unrounded ones
-          uint32_t w[32];
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const int x = 2 * h + e / 16, y = (2 * e) % 32;
-            float2 a = fma2(make_float2(__uint_as_float(s[x][y]), __uint_as_float(s[x][y + 1])), scale2, sub2);
-            a.x = ex2(a.x);
-            a.y = ex2(a.y);
-            sum[e & 1] = add2(sum[e & 1], a);
-            w[e] = Elem<T>::pack(a.x, a.y);
-          }
-          tmem_st32(ts + 32 * h, w);
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&bar_p[g][h]));
+          for (int e = 0; e < 32; ++e) u[e] = weights(e);
+          tmem_st32(ts, u);
         }
+        uint32_t u[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) u[e] = weights(32 + e);
+        tmem_st16(ts + 32, u);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bar_p[g][0]));
+#pragma unroll
+        for (int e = 0; e < 16; ++e) u[e] = weights(48 + e);
+        tmem_st16(ts + 48, u);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bar_p[g][1]));
         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       }
+      if (!ok) break;
       // ---- the row's result
-      if (nt > 0 && ok) {
-        ok = warp_wait(smem_u32(&bar_o[g]), 0);
+      if (w.nt > 0) {
+        if (!(ok = warp_wait(smem_u32(&bar_o[g]), no++ & 1))) break;
         tc_fence_after();
       }
-      if (ok) {
-        const int tok = tok0 + g * p.rp + (have ? r / p.group : 0), head = kvh * p.group + (have ? r % p.group : 0);
+      if (odd_s[it & 3]) add_nonfinite<T, HD>(p, w, pos, lo, sinks, to);
+      const int tok = w.tok0 + g * p.rp + r_pos, head = w.kvh * p.group + r_head;
+      // 128 bytes of each of the warp's 32 rows at a time go through shared memory
+      // (16-byte chunk c of a row at chunk c ^ (row & 7)), so that eight lanes
+      // write a row's 128 bytes together. row_at: this lane's row, in bytes, or -1.
+      auto write_out = [&](uint8_t* out, long long row_at) {
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int row = 4 * k + lane / 8, c = lane % 8;
+          const long long at = __shfl_sync(0xffffffffu, row_at, row);
+          const uint4 v = lds128(stage + row * 128 + ((c ^ (row & 7)) << 4));
+          if (at >= 0) *reinterpret_cast<uint4*>(out + at + c * 16) = v;
+        }
+        __syncwarp();
+      };
+      auto put = [&](int c, uint4 v) { sts128(stage + lane * 128 + ((c ^ (lane & 7)) << 4), v); };
+      if (p.slices == 1) {
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        const bool odd = odd_s;
-        const long long at = ((long long)slice * p.T + tok) * p.nq + head;
-        if (p.slices > 1 && have) p.part_ml[at] = make_float2(nt > 0 ? m : -INFINITY, l);
+        const long long row_at = have ? (tok * p.o_t + head * p.o_h) * 2 : -1ll;
 #pragma unroll 1
-        for (int x = 0; x < HD / 32; ++x) {
-          uint32_t o[32];
-          if (nt > 0) {
-            tmem_ld32(to + 32 * x, o);
+        for (int c0 = 0; c0 < HD; c0 += 64) {
+          uint32_t o[2][32];
+          if (w.nt > 0) {
+            tmem_ld32(to + c0, o[0]);
+            tmem_ld32(to + c0 + 32, o[1]);
             tmem_wait_ld();
-            tmem_regs_ready(o);
+            tmem_regs_ready(o[0]);
+            tmem_regs_ready(o[1]);
           } else {
-            if (p.slices > 1) break;   // nothing of this slice is read
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = 0u;
+            for (int e = 0; e < 64; ++e) o[e / 32][e % 32] = 0u;
           }
-          if (odd && have) {
-            // the values that were cleared and that this row sees
-            for (int i = 0; i < nt; ++i) {
-              const int key0 = key_of(i);
-              if (!(key0 + kPmKeys - 1 > pos0 || (windowed && key0 <= last - p.window))) continue;
-              for (int key = key0; key < key0 + kPmKeys; ++key) {
-                if (!sees(key)) continue;
-                const int page = page_id(p.c, b, key);
-                if (page < 0) continue;
-                const T* v = static_cast<const T*>(p.c.v) + page * p.c.vp + kvh * p.c.vh +
-                             (key & (p.c.page_size - 1)) * p.c.vs + 32 * x;
 #pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                  const float f = static_cast<float>(v[e]);
-                  if (!isfinite(f)) o[e] = __float_as_uint(__uint_as_float(o[e]) + f);
-                }
-              }
-            }
+          for (int c = 0; c < 8; ++c) {
+            uint32_t u[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              u[e] = Elem<T>::pack(__uint_as_float(o[c / 4][8 * (c % 4) + 2 * e]) * inv,
+                                   __uint_as_float(o[c / 4][8 * (c % 4) + 2 * e + 1]) * inv);
+            put(c, make_uint4(u[0], u[1], u[2], u[3]));
           }
-          if (!have) continue;
-          if (p.slices > 1) {
-            float4* dst = reinterpret_cast<float4*>(p.part_o + at * HD + 32 * x);
+          write_out(static_cast<uint8_t*>(p.out) + c0 * 2, row_at);
+        }
+      } else {
+        const long long part = ((long long)w.slice * p.T + tok) * p.nq + head;
+        if (have) p.part_ml[part] = make_float2(w.nt > 0 ? m : -INFINITY, l);
+        if (w.nt == 0) continue;   // nothing else of this slice is read
+#pragma unroll 1
+        for (int c0 = 0; c0 < HD; c0 += 32) {
+          uint32_t o[32];
+          tmem_ld32(to + c0, o);
+          tmem_wait_ld();
+          tmem_regs_ready(o);
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              dst[e] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]),
-                                   __uint_as_float(o[4 * e + 3]));
-          } else {
-            uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + tok * p.o_t + head * p.o_h + 32 * x);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              uint32_t u[4];
-#pragma unroll
-              for (int f = 0; f < 4; ++f)
-                u[f] = Elem<T>::pack(__uint_as_float(o[8 * e + 2 * f]) * inv, __uint_as_float(o[8 * e + 2 * f + 1]) * inv);
-              dst[e] = make_uint4(u[0], u[1], u[2], u[3]);
-            }
-          }
+          for (int c = 0; c < 8; ++c) put(c, make_uint4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]));
+          write_out(reinterpret_cast<uint8_t*>(p.part_o) + c0 * 4, have ? part * HD * 4 : -1ll);
         }
       }
     }
