@@ -92,6 +92,25 @@ LW_DEV void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+// Two fp32 operations in one instruction.
+LW_DEV uint64_t as_u64(float2 v) { return *reinterpret_cast<uint64_t*>(&v); }
+LW_DEV float2 as_f2(uint64_t v) { return *reinterpret_cast<float2*>(&v); }
+LW_DEV float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t y;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(as_u64(a)), "l"(as_u64(b)), "l"(as_u64(c)));
+  return as_f2(y);
+}
+LW_DEV float2 add2(float2 a, float2 b) {
+  uint64_t y;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(as_u64(a)), "l"(as_u64(b)));
+  return as_f2(y);
+}
+LW_DEV float2 mul2(float2 a, float2 b) {
+  uint64_t y;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(as_u64(a)), "l"(as_u64(b)));
+  return as_f2(y);
+}
+
 // 2^x (a result below the normal range is 0).
 LW_DEV float ex2(float x) {
   float y;

@@ -146,20 +146,6 @@ LW_DEV float max3(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
-// Two fp32 operations in one instruction.
-LW_DEV uint64_t as_u64(float2 v) { return *reinterpret_cast<uint64_t*>(&v); }
-LW_DEV float2 as_f2(uint64_t v) { return *reinterpret_cast<float2*>(&v); }
-LW_DEV float2 fma2(float2 a, float2 b, float2 c) {
-  uint64_t y;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(as_u64(a)), "l"(as_u64(b)), "l"(as_u64(c)));
-  return as_f2(y);
-}
-LW_DEV float2 add2(float2 a, float2 b) {
-  uint64_t y;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(as_u64(a)), "l"(as_u64(b)));
-  return as_f2(y);
-}
-
 // Zeros in the place of the infinities and NaNs of a row of V (128 bytes in each half).
 template <typename T>
 __device__ __noinline__ void clear_nonfinite(uint8_t* row, int halves, int half_bytes) {

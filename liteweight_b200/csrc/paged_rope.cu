@@ -4,13 +4,15 @@
 //   y = x * rsqrt(mean(x^2) + eps) * w,   o[d] = y[d] cos[p][d] + r[d] sin[p][d],
 //   r = (-y[hd/2:], y[:hd/2])
 //
-// A group of hd / 16 lanes takes one token's run of up to HPG heads (queries,
-// then keys, then values): each lane holds dims 8j .. 8j+7 and their rotation
+// A group of hd / 16 lanes takes one token's run of up to HPG heads of one kind
+// (queries, keys or values): each lane holds dims 8j .. 8j+7 and their rotation
 // partners hd/2 + 8j .. + 7, so a head is two 16-byte loads and two 16-byte
 // stores a lane, the rotation needs no exchange, and the mean is log2(hd / 16)
-// shuffles. The angle's cosines and sines are loaded once per run. All of it in
-// fp32 with one rounding at the store. Memory bound: every element is read
-// once and written once.
+// shuffles. Weight and angle make four factors per pair, formed once per run:
+//   o_lo = r (x_lo [w_lo cos_lo] - x_hi [w_hi sin_lo]),  r = rsqrt(mean + eps)
+//   o_hi = r (x_hi [w_hi cos_hi] + x_lo [w_lo sin_hi])
+// All of it in fp32 with one rounding at the store. Memory bound: every element
+// is read once and written once.
 #include "paged.cuh"
 
 namespace lw {
@@ -20,7 +22,7 @@ struct RopeParams {
   const void *q, *k, *v;
   long long q_t, q_h, k_t, k_h, v_t, v_h, o_t, o_h;
   void* out;
-  int T, nq, chunks;   // runs of heads per token
+  int T, nq, q_runs, kv_runs;   // runs of heads per token: q_runs + 2 * kv_runs
   const int* off;
   const void *cos, *sin;
   long long rope_stride;
@@ -30,70 +32,68 @@ struct RopeParams {
   int zero_tail;
 };
 
+// 8 elements as four pairs.
 template <typename T>
-LW_DEV void load8(const T* p, float (&f)[8]) {
-  const uint4 u = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 x = Elem<T>::unpack(w[i]);
-    f[2 * i] = x.x;
-    f[2 * i + 1] = x.y;
-  }
+LW_DEV void unpack8(const uint4& u, float2 (&f)[4]) {
+  f[0] = Elem<T>::unpack(u.x);
+  f[1] = Elem<T>::unpack(u.y);
+  f[2] = Elem<T>::unpack(u.z);
+  f[3] = Elem<T>::unpack(u.w);
+}
+template <typename T>
+LW_DEV void load8(const T* p, float2 (&f)[4]) {
+  unpack8<T>(*reinterpret_cast<const uint4*>(p), f);
 }
 template <>
-LW_DEV void load8<float>(const float* p, float (&f)[8]) {
+LW_DEV void load8<float>(const float* p, float2 (&f)[4]) {
   const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-  f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w;
-  f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+  f[0] = make_float2(a.x, a.y);
+  f[1] = make_float2(a.z, a.w);
+  f[2] = make_float2(b.x, b.y);
+  f[3] = make_float2(b.z, b.w);
 }
 
-template <typename T>
-LW_DEV void unpack8(const uint4& u, float (&f)[8]) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 x = Elem<T>::unpack(w[i]);
-    f[2 * i] = x.x;
-    f[2 * i + 1] = x.y;
-  }
-}
-
-template <typename T>
-LW_DEV uint4 pack8(const float (&f)[8]) {
-  return make_uint4(Elem<T>::pack(f[0], f[1]), Elem<T>::pack(f[2], f[3]), Elem<T>::pack(f[4], f[5]),
-                    Elem<T>::pack(f[6], f[7]));
+// 16 bytes that are read once: not kept in L1, where the tables and weights are.
+LW_DEV uint4 load_once(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p)
+               : "memory");
+  return v;
 }
 
 constexpr int kRopeThreads = 256;
 
 // T: element type; TT: type of the rotation table; HPG: heads per run.
 template <typename T, typename TT, int HD, int HPG>
-__global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_kernel(const RopeParams p) {
+__global__ void __launch_bounds__(kRopeThreads, 2) qk_norm_rope_kernel(const RopeParams p) {
   constexpr int LPR = HD / 16;   // lanes per head
   pdl_wait();
   pdl_launch_dependents();
-  const int j = threadIdx.x % LPR;
+  const int j = threadIdx.x % LPR, runs = p.q_runs + 2 * p.kv_runs;
   const long long item = (long long)blockIdx.x * (kRopeThreads / LPR) + threadIdx.x / LPR;
-  const long long t64 = item / p.chunks;
+  const long long t64 = item / runs;
   if (t64 >= p.T) return;   // whole groups: shuffles below stay within a group
-  const int t = (int)t64, h0 = (int)(item - t64 * p.chunks) * HPG;
-  const int heads = p.nq + 2 * p.c.nkv;
-  const unsigned gmask = (LPR == 32 ? 0xffffffffu : ((1u << LPR) - 1u)) << ((threadIdx.x & 31) / LPR * LPR);
+  const int t = (int)t64;
+  int run = (int)(item - t64 * runs);
+  const int kind = run < p.q_runs ? 0 : run < p.q_runs + p.kv_runs ? 1 : 2;   // queries, keys, values
+  run -= kind == 0 ? 0 : kind == 1 ? p.q_runs : p.q_runs + p.kv_runs;
+  const int h0 = run * HPG, n = min(HPG, (kind ? p.c.nkv : p.nq) - h0);
+  const unsigned gmask = ((1u << LPR) - 1u) << ((threadIdx.x & 31) / LPR * LPR);
   const int d_lo = 8 * j, d_hi = HD / 2 + 8 * j;
 
   // the run's heads, all loads in flight before the first use
   uint4 lo[HPG], hi[HPG];
+  {
+    const long long st = kind == 0 ? p.q_t : kind == 1 ? p.k_t : p.v_t, sh = kind == 0 ? p.q_h : kind == 1 ? p.k_h : p.v_h;
+    const T* src = static_cast<const T*>(kind == 0 ? p.q : kind == 1 ? p.k : p.v) + t * st + h0 * sh;
 #pragma unroll
-  for (int i = 0; i < HPG; ++i) {
-    const int h = h0 + i;
-    if (h >= heads) break;
-    const T* src;
-    if (h < p.nq) src = static_cast<const T*>(p.q) + t * p.q_t + h * p.q_h;
-    else if (h < p.nq + p.c.nkv) src = static_cast<const T*>(p.k) + t * p.k_t + (h - p.nq) * p.k_h;
-    else src = static_cast<const T*>(p.v) + t * p.v_t + (h - p.nq - p.c.nkv) * p.v_h;
-    lo[i] = *reinterpret_cast<const uint4*>(src + d_lo);
-    hi[i] = *reinterpret_cast<const uint4*>(src + d_hi);
+    for (int i = 0; i < HPG; ++i) {
+      if (i >= n) break;
+      lo[i] = load_once(src + i * sh + d_lo);
+      hi[i] = load_once(src + i * sh + d_hi);
+    }
   }
 
   const int b = p.off ? row_sequence(p.off, p.c.B, t) : t;
@@ -102,90 +102,92 @@ __global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_kernel(const RopePa
     const int len = p.c.lens[b];
     pos = p.off ? len - p.off[b + 1] + t : len - 1;
   }
-  const bool real = b >= 0 && pos >= 0;   // the row is a token of a sequence
-  const bool turns = real && pos < p.rope_rows;
-  if (!turns) {
+  T* dst = kind == 0 ? static_cast<T*>(p.out) + t * p.o_t + h0 * p.o_h : nullptr;
+  long long dh = p.o_h;
+  if (b < 0 || pos < 0 || pos >= p.rope_rows) {   // a row of no sequence, or a position that there is not
     // past the table, or more new tokens than the length counts
-    if ((real || (b >= 0 && p.off)) && j == 0) lw_record_error(LW_ERR_BAD_INDEX);
-    if (p.zero_tail) {
-#pragma unroll
-      for (int i = 0; i < HPG; ++i) {
-        if (h0 + i >= p.nq) break;
-        T* dst = static_cast<T*>(p.out) + t * p.o_t + (h0 + i) * p.o_h;
-        *reinterpret_cast<uint4*>(dst + d_lo) = make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(dst + d_hi) = make_uint4(0, 0, 0, 0);
+    if (b >= 0 && (pos >= 0 || p.off) && j == 0) lw_record_error(LW_ERR_BAD_INDEX);
+    if (kind == 0 && p.zero_tail)
+#pragma unroll 1
+      for (int i = 0; i < n; ++i) {
+        *reinterpret_cast<uint4*>(dst + i * dh + d_lo) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(dst + i * dh + d_hi) = make_uint4(0, 0, 0, 0);
       }
-    }
     return;
   }
-  // where the token is kept (only the runs that reach keys or values ask)
-  long long k_at = -1, v_at = -1;
-  if (h0 + HPG > p.nq) {
+  if (kind) {   // where the token is kept
     const int page = (pos >> p.c.page_shift) < p.c.table_width ? page_id(p.c, b, pos) : -1;
-    if (page >= 0) {
-      const int slot = pos & (p.c.page_size - 1);
-      k_at = page * p.c.kp + slot * p.c.ks;
-      v_at = page * p.c.vp + slot * p.c.vs;
-    } else if (j == 0) {
-      lw_record_error(LW_ERR_BAD_INDEX);
+    if (page < 0) {
+      if (j == 0) lw_record_error(LW_ERR_BAD_INDEX);
+      return;
+    }
+    const long long slot = pos & (p.c.page_size - 1);
+    if (kind == 1) dst = static_cast<T*>(p.c.k) + page * p.c.kp + slot * p.c.ks + h0 * p.c.kh, dh = p.c.kh;
+    else dst = static_cast<T*>(p.c.v) + page * p.c.vp + slot * p.c.vs + h0 * p.c.vh, dh = p.c.vh;
+    if (kind == 2) {   // values are kept as they are
+#pragma unroll
+      for (int i = 0; i < HPG; ++i) {
+        if (i >= n) break;
+        *reinterpret_cast<uint4*>(dst + i * dh + d_lo) = lo[i];
+        *reinterpret_cast<uint4*>(dst + i * dh + d_hi) = hi[i];
+      }
+      return;
     }
   }
-  float c_lo[8], c_hi[8], s_lo[8], s_hi[8];
+  // factors of the pairs: own and partner's, for the low and the high half
+  float2 own_lo[4], own_hi[4], par_lo[4], par_hi[4];
   {
     const TT* cs = static_cast<const TT*>(p.cos) + pos * p.rope_stride;
     const TT* sn = static_cast<const TT*>(p.sin) + pos * p.rope_stride;
-    load8(cs + d_lo, c_lo);
-    load8(cs + d_hi, c_hi);
-    load8(sn + d_lo, s_lo);
-    load8(sn + d_hi, s_hi);
+    load8(cs + d_lo, own_lo);
+    load8(cs + d_hi, own_hi);
+    load8(sn + d_lo, par_lo);
+    load8(sn + d_hi, par_hi);
+  }
+  const T* w = static_cast<const T*>(kind ? p.kw : p.qw);
+  const float2 minus = make_float2(-1.f, -1.f);
+  if (w) {
+    float2 w_lo[4], w_hi[4];
+    load8(w + d_lo, w_lo);
+    load8(w + d_hi, w_hi);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      own_lo[e] = mul2(own_lo[e], w_lo[e]);
+      own_hi[e] = mul2(own_hi[e], w_hi[e]);
+      par_lo[e] = mul2(mul2(par_lo[e], minus), w_hi[e]);
+      par_hi[e] = mul2(par_hi[e], w_lo[e]);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) par_lo[e] = mul2(par_lo[e], minus);
   }
 #pragma unroll
   for (int i = 0; i < HPG; ++i) {
-    const int h = h0 + i;
-    if (h >= heads) break;
-    if (h >= p.nq + p.c.nkv) {   // values are kept as they are
-      if (v_at >= 0) {
-        T* dst = static_cast<T*>(p.c.v) + v_at + (h - p.nq - p.c.nkv) * p.c.vh;
-        *reinterpret_cast<uint4*>(dst + d_lo) = lo[i];
-        *reinterpret_cast<uint4*>(dst + d_hi) = hi[i];
-      }
-      continue;
-    }
-    float x_lo[8], x_hi[8];
+    if (i >= n) break;
+    float2 x_lo[4], x_hi[4];
     unpack8<T>(lo[i], x_lo);
     unpack8<T>(hi[i], x_hi);
-    const T* w = static_cast<const T*>(h < p.nq ? p.qw : p.kw);
+    float r = 1.f;
     if (w) {
-      float ss = 0.f;
+      float2 ss = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(x_lo[e], x_lo[e], fmaf(x_hi[e], x_hi[e], ss));
+      for (int e = 0; e < 4; ++e) ss = fma2(x_lo[e], x_lo[e], fma2(x_hi[e], x_hi[e], ss));
+      float sum = ss.x + ss.y;
 #pragma unroll
-      for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(gmask, ss, o);
-      const float r = rsqrtf(ss * (1.0f / HD) + p.eps);
-      float w_lo[8], w_hi[8];
-      load8(w + d_lo, w_lo);
-      load8(w + d_hi, w_hi);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x_lo[e] = x_lo[e] * r * w_lo[e];
-        x_hi[e] = x_hi[e] * r * w_hi[e];
-      }
+      for (int o = LPR / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(gmask, sum, o);
+      r = rsqrtf(sum * (1.0f / HD) + p.eps);
     }
-    float y_lo[8], y_hi[8];
+    const float2 r2 = make_float2(r, r);
+    uint32_t y_lo[4], y_hi[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      y_lo[e] = x_lo[e] * c_lo[e] - x_hi[e] * s_lo[e];
-      y_hi[e] = x_hi[e] * c_hi[e] + x_lo[e] * s_hi[e];
+    for (int e = 0; e < 4; ++e) {
+      const float2 a = mul2(r2, fma2(x_lo[e], own_lo[e], mul2(x_hi[e], par_lo[e])));
+      const float2 c = mul2(r2, fma2(x_hi[e], own_hi[e], mul2(x_lo[e], par_hi[e])));
+      y_lo[e] = Elem<T>::pack(a.x, a.y);
+      y_hi[e] = Elem<T>::pack(c.x, c.y);
     }
-    T* dst;
-    if (h < p.nq) {
-      dst = static_cast<T*>(p.out) + t * p.o_t + h * p.o_h;
-    } else {
-      if (k_at < 0) continue;
-      dst = static_cast<T*>(p.c.k) + k_at + (h - p.nq) * p.c.kh;
-    }
-    *reinterpret_cast<uint4*>(dst + d_lo) = pack8<T>(y_lo);
-    *reinterpret_cast<uint4*>(dst + d_hi) = pack8<T>(y_hi);
+    *reinterpret_cast<uint4*>(dst + i * dh + d_lo) = make_uint4(y_lo[0], y_lo[1], y_lo[2], y_lo[3]);
+    *reinterpret_cast<uint4*>(dst + i * dh + d_hi) = make_uint4(y_hi[0], y_hi[1], y_hi[2], y_hi[3]);
   }
 }
 
@@ -196,10 +198,10 @@ namespace {
 template <typename T, typename TT, int HD>
 cudaError_t rope_launch(lw::RopeParams& p, cudaStream_t s, bool pdl) {
   constexpr int groups = lw::kRopeThreads / (HD / 16);
-  const int heads = p.nq + 2 * p.c.nkv;
   auto blocks = [&](int hpg) {
-    p.chunks = (heads + hpg - 1) / hpg;
-    return ((long long)p.T * p.chunks + groups - 1) / groups;
+    p.q_runs = (p.nq + hpg - 1) / hpg;
+    p.kv_runs = (p.c.nkv + hpg - 1) / hpg;
+    return ((long long)p.T * (p.q_runs + 2 * p.kv_runs) + groups - 1) / groups;
   };
   // A run of 8 heads shares one load of the angles and keeps 16 loads in flight
   // a lane; a launch too small to give every SM work takes single heads.
