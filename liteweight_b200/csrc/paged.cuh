@@ -4,6 +4,8 @@
 
 #include <cuda_bf16.h>
 
+#include <atomic>
+
 #include "lw_common.cuh"
 
 namespace lw {
@@ -79,6 +81,12 @@ LW_DEV void ldmatrix_x4_t(uint32_t addr, uint32_t (&r)[4]) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr)
                : "memory");
+}
+
+LW_DEV float2 lds_f2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
 }
 
 // 16 bytes global -> shared, zeros instead when !valid (src is not read then).
@@ -215,6 +223,21 @@ inline lw::PagedView view_of(const lw_paged_cache& c) {
   v.table_width = c.table_width;
   v.lens = c.kv_lens;
   return v;
+}
+
+// Lets a kernel use `bytes` of dynamic shared memory on the current device (asked
+// once per kernel and device: it costs as much as a quarter of a launch).
+template <auto kKernel>
+inline cudaError_t allow_smem(int bytes) {
+  static std::atomic<unsigned long long> done{0};   // bit per device
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const unsigned long long bit = dev >= 0 && dev < 64 ? 1ull << dev : 0ull;
+  if (bit & done.load(std::memory_order_relaxed)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
 }
 
 inline int sm_count() {

@@ -5,8 +5,8 @@
 //   position p = kv_lens[b] - 1 sees.
 //
 // Bound by reading the visible keys and values once. The work is cut into
-// tiles of 16 consecutive token positions (one page each: a page is a multiple
-// of 16 slots) of one item = (sequence, kv head, block of up to ROWS query
+// tiles of 16 (head_dim 128) or 32 (64) consecutive token positions, 8 KB of keys
+// and values, of one item = (sequence, kv head, block of up to ROWS query
 // heads of its group). A warp streams tiles through a private ring of
 // shared-memory stages (cp.async, no CTA barrier), computes S = Q K^T and
 // O += P V with mma.sync (the query heads are the MMA's rows, so K and V are
@@ -35,7 +35,6 @@ namespace lw {
 
 constexpr int kPdWarps = 8;
 constexpr int kPdThreads = kPdWarps * 32;
-constexpr int kPdTile = 16;      // keys per tile
 
 struct PagedDecodeParams {
   PagedView c;
@@ -53,25 +52,32 @@ struct PagedDecodeParams {
 struct TileSpan {
   int len, lo, sinks;   // keys [lo, len) and [0, sinks) are visible
   int ns, w0, nt;
-  LW_DEV int key0(int tile) const { return (tile < ns ? tile : w0 + tile - ns) * kPdTile; }
 };
 
+template <int TILE>
 LW_DEV TileSpan tile_span(const PagedDecodeParams& p, int len) {
   TileSpan s;
   s.len = len;
   s.lo = window_start(len - 1, p.window);
   s.sinks = min(p.sinks, s.lo);
-  s.w0 = s.lo / kPdTile;
-  s.ns = min((s.sinks + kPdTile - 1) / kPdTile, s.w0);
-  s.nt = len > 0 ? s.ns + (len + kPdTile - 1) / kPdTile - s.w0 : 0;
+  s.w0 = s.lo / TILE;
+  s.ns = min((s.sinks + TILE - 1) / TILE, s.w0);
+  s.nt = len > 0 ? s.ns + (len + TILE - 1) / TILE - s.w0 : 0;
   return s;
+}
+// First key of a span's tile.
+template <int TILE>
+LW_DEV int tile_key(const TileSpan& s, int tile) {
+  return (tile < s.ns ? tile : s.w0 + tile - s.ns) * TILE;
 }
 
 // Sizes of a kernel's shared memory: a ring per warp, then pieces [warps][ROWS][HD + 8]
 // (accumulator, maximum, sum; the stride keeps the fragment stores off each other's banks).
 template <int HD, int ROWS>
 struct DecodeShape {
-  static constexpr int kTileBytes = kPdTile * HD * 2;           // K or V of a tile
+  static constexpr int kTile = 2048 / HD;                       // keys per tile
+  static constexpr int kGroups = kTile / 16;                    // of 16 keys: one page each
+  static constexpr int kTileBytes = kTile * HD * 2;             // K or V of a tile
   static constexpr int kRing = ROWS == 8 ? 24576 : 16384;       // per warp
   static constexpr int kStages = kRing / (2 * kTileBytes);
   static constexpr int kStride = HD + 8;
@@ -111,37 +117,45 @@ struct WarpItem {
     for (int r = 0; r < R; ++r) m[r] = -INFINITY, l[r] = 0.f;
   }
 
-  // Keys key0 .. key0 + 15 of the stage at `kt` (K tile, then V tile; 16-byte
-  // chunk c of row r at chunk c ^ (r & 7)).
-  LW_DEV void tile(const PagedDecodeParams& p, const TileSpan& sp, int key0, bool kept, uint32_t kt, int lane) {
+  // The keys from key0 on, in the stage at `kt` (K tile, then V tile; 16-byte chunk
+  // c of row r at chunk c ^ (r & 7)); bit i of `lost`: the 16-key group i is hidden.
+  LW_DEV void tile(const PagedDecodeParams& p, const TileSpan& sp, int key0, uint32_t lost, uint32_t kt, int lane) {
+    constexpr int N = S::kTile / 8;   // score fragments of 8 keys
     const int t = lane & 3;
-    float sc[2][4] = {};
+    float sc[N][4];
+#pragma unroll
+    for (int n = 0; n < N; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
     {
       // matrices of 8 keys x 8 dims: (keys 0-7 | 8-15) x (dims 0-7 | 8-15) of a k-step
-      const int r = (lane >> 4) * 8 + (lane & 7), cb = (lane >> 3) & 1;
+      const int r0 = (lane >> 4) * 8 + (lane & 7), cb = (lane >> 3) & 1;
 #pragma unroll
-      for (int k = 0; k < HD / 16; ++k) {
-        uint32_t b[4];
-        ldmatrix_x4(kt + (uint32_t)(r * (HD * 2) + (((2 * k + cb) ^ (r & 7)) << 4)), b);
-        const uint32_t a1 = R == 2 ? qa[k][R - 1] : 0u, a3 = R == 2 ? qa[k][2 * R - 1] : 0u;
-        mma_16816<T>(sc[0], qa[k][0], a1, qa[k][R], a3, b[0], b[1]);
-        mma_16816<T>(sc[1], qa[k][0], a1, qa[k][R], a3, b[2], b[3]);
-      }
+      for (int k = 0; k < HD / 16; ++k)
+#pragma unroll
+        for (int x = 0; x < S::kGroups; ++x) {
+          const int r = 16 * x + r0;
+          uint32_t b[4];
+          ldmatrix_x4(kt + (uint32_t)(r * (HD * 2) + (((2 * k + cb) ^ (r & 7)) << 4)), b);
+          const uint32_t a1 = R == 2 ? qa[k][R - 1] : 0u, a3 = R == 2 ? qa[k][2 * R - 1] : 0u;
+          mma_16816<T>(sc[2 * x], qa[k][0], a1, qa[k][R], a3, b[0], b[1]);
+          mma_16816<T>(sc[2 * x + 1], qa[k][0], a1, qa[k][R], a3, b[2], b[3]);
+        }
     }
-    const bool whole = kept && key0 + kPdTile <= sp.len && (key0 >= sp.lo || key0 + kPdTile <= sp.sinks);
+    const bool whole = !lost && key0 + S::kTile <= sp.len && (key0 >= sp.lo || key0 + S::kTile <= sp.sinks);
     if (!whole) {
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < N; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int key = key0 + n * 8 + 2 * t + (e & 1);
-          if (!(kept && key < sp.len && (key >= sp.lo || key < sp.sinks))) sc[n][e] = -INFINITY;
+          if (((lost >> (n / 2)) & 1u) || key >= sp.len || (key < sp.lo && key >= sp.sinks)) sc[n][e] = -INFINITY;
         }
     }
     float corr[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      float mx = fmaxf(fmaxf(sc[0][2 * r], sc[0][2 * r + 1]), fmaxf(sc[1][2 * r], sc[1][2 * r + 1]));
+      float mx = fmaxf(sc[0][2 * r], sc[0][2 * r + 1]);
+#pragma unroll
+      for (int n = 1; n < N; ++n) mx = fmaxf(mx, fmaxf(sc[n][2 * r], sc[n][2 * r + 1]));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
       const float mn = fmaxf(m[r], mx * p.scale_log2);
@@ -150,7 +164,7 @@ struct WarpItem {
       m[r] = mn;
       float sum = 0.f;
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < N; ++n)
 #pragma unroll
         for (int e = 2 * r; e < 2 * r + 2; ++e) {
           sc[n][e] = ex2(fmaf(sc[n][e], p.scale_log2, -base));
@@ -158,11 +172,6 @@ struct WarpItem {
         }
       l[r] = fmaf(l[r], corr[r], sum);
     }
-    // the weights lie in [0, 1]: rounded to T for the second product, half a
-    // step each, averaged over the keys; their sum stays in fp32
-    const uint32_t a0 = Elem<T>::pack(sc[0][0], sc[0][1]), a2 = Elem<T>::pack(sc[1][0], sc[1][1]);
-    const uint32_t a1 = R == 2 ? Elem<T>::pack(sc[0][2], sc[0][3]) : 0u;
-    const uint32_t a3 = R == 2 ? Elem<T>::pack(sc[1][2], sc[1][3]) : 0u;
 #pragma unroll
     for (int i = 0; i < HD / 8; ++i) {
       o[i][0] *= corr[0];
@@ -173,13 +182,22 @@ struct WarpItem {
       }
     }
     const uint32_t vt = kt + S::kTileBytes;
-    const int r = ((lane >> 3) & 1) * 8 + (lane & 7), cb = lane >> 4;
+    const int r0 = ((lane >> 3) & 1) * 8 + (lane & 7), cb = lane >> 4;
 #pragma unroll
-    for (int d = 0; d < HD / 16; ++d) {
-      uint32_t b[4];
-      ldmatrix_x4_t(vt + (uint32_t)(r * (HD * 2) + (((2 * d + cb) ^ (r & 7)) << 4)), b);
-      mma_16816<T>(o[2 * d], a0, a1, a2, a3, b[0], b[1]);
-      mma_16816<T>(o[2 * d + 1], a0, a1, a2, a3, b[2], b[3]);
+    for (int x = 0; x < S::kGroups; ++x) {
+      // the weights lie in [0, 1]: rounded to T for the second product, half a
+      // step each, averaged over the keys; their sum stays in fp32
+      const uint32_t a0 = Elem<T>::pack(sc[2 * x][0], sc[2 * x][1]), a2 = Elem<T>::pack(sc[2 * x + 1][0], sc[2 * x + 1][1]);
+      const uint32_t a1 = R == 2 ? Elem<T>::pack(sc[2 * x][2], sc[2 * x][3]) : 0u;
+      const uint32_t a3 = R == 2 ? Elem<T>::pack(sc[2 * x + 1][2], sc[2 * x + 1][3]) : 0u;
+      const int r = 16 * x + r0;
+#pragma unroll
+      for (int d = 0; d < HD / 16; ++d) {
+        uint32_t b[4];
+        ldmatrix_x4_t(vt + (uint32_t)(r * (HD * 2) + (((2 * d + cb) ^ (r & 7)) << 4)), b);
+        mma_16816<T>(o[2 * d], a0, a1, a2, a3, b[0], b[1]);
+        mma_16816<T>(o[2 * d + 1], a0, a1, a2, a3, b[2], b[3]);
+      }
     }
   }
 
@@ -221,24 +239,38 @@ struct WarpItem {
   }
 };
 
-// The warp's copy of a tile into a ring stage: zeros for keys nobody sees.
+// The warp's copy of a tile into a ring stage, zeros for keys nobody sees. Returns
+// the 16-key groups whose page id is outside the pool: their keys are hidden.
 template <typename T, int HD, int ROWS>
-LW_DEV void copy_tile(const PagedDecodeParams& p, const TileSpan& sp, int key0, int page, int kvh, uint32_t dst,
-                      int lane) {
+LW_DEV uint32_t copy_tile(const PagedDecodeParams& p, const TileSpan& sp, int b, int key0, int kvh, uint32_t dst,
+                          int lane) {
   using S = DecodeShape<HD, ROWS>;
-  constexpr int CPR = HD / 8, ROWS_PER_INSTR = 32 / CPR, COPIES = kPdTile / ROWS_PER_INSTR;
+  constexpr int CPR = HD / 8, ROWS_PER_INSTR = 32 / CPR, COPIES = 16 / ROWS_PER_INSTR;
   const int c_row = lane / CPR, c_chunk = lane % CPR;
-  const int slot0 = key0 & (p.c.page_size - 1);
-  const T* kp = static_cast<const T*>(p.c.k) + page * p.c.kp + kvh * p.c.kh + slot0 * p.c.ks + c_chunk * 8;
-  const T* vp = static_cast<const T*>(p.c.v) + page * p.c.vp + kvh * p.c.vh + slot0 * p.c.vs + c_chunk * 8;
+  int page[S::kGroups];
+  uint32_t lost = 0;
 #pragma unroll
-  for (int i = 0; i < COPIES; ++i) {
-    const int r = c_row + i * ROWS_PER_INSTR, key = key0 + r;
-    const bool ok = page >= 0 && key < sp.len && (key >= sp.lo || key < sp.sinks);
-    const uint32_t at = dst + (uint32_t)(r * (HD * 2) + ((c_chunk ^ (r & 7)) << 4));
-    cp_async16(at, ok ? kp + r * p.c.ks : static_cast<const T*>(p.q), ok);
-    cp_async16(at + S::kTileBytes, ok ? vp + r * p.c.vs : static_cast<const T*>(p.q), ok);
+  for (int x = 0; x < S::kGroups; ++x) {
+    const int first = key0 + 16 * x;   // a group may lie outside what is seen: its table entry is not read
+    const bool seen = S::kGroups == 1 || (first < sp.len && (first + 16 > sp.lo || first < sp.sinks));
+    page[x] = seen ? page_id(p.c, b, first) : 0;
+    if (page[x] < 0) lost |= 1u << x;
   }
+#pragma unroll
+  for (int x = 0; x < S::kGroups; ++x) {
+    const int first = key0 + 16 * x, slot0 = first & (p.c.page_size - 1);
+    const T* kp = static_cast<const T*>(p.c.k) + page[x] * p.c.kp + kvh * p.c.kh + slot0 * p.c.ks + c_chunk * 8;
+    const T* vp = static_cast<const T*>(p.c.v) + page[x] * p.c.vp + kvh * p.c.vh + slot0 * p.c.vs + c_chunk * 8;
+#pragma unroll
+    for (int i = 0; i < COPIES; ++i) {
+      const int r = c_row + i * ROWS_PER_INSTR, key = first + r;
+      const bool ok = page[x] >= 0 && key < sp.len && (key >= sp.lo || key < sp.sinks);
+      const uint32_t at = dst + (uint32_t)((16 * x + r) * (HD * 2) + ((c_chunk ^ (r & 7)) << 4));
+      cp_async16(at, ok ? kp + r * p.c.ks : static_cast<const T*>(p.q), ok);
+      cp_async16(at + S::kTileBytes, ok ? vp + r * p.c.vs : static_cast<const T*>(p.q), ok);
+    }
+  }
+  return lost;
 }
 
 // A place on the line of tiles: sequence b, its span, item (kv head, head block) within it.
@@ -265,6 +297,7 @@ __global__ void __launch_bounds__(kPdThreads, 1) paged_decode_kernel(const Paged
   float* head_piece = reinterpret_cast<float*>(smem + kPdWarps * S::kRing) + warp * S::kPiece;
   float* tail_piece = reinterpret_cast<float*>(smem + warp * S::kRing);   // the ring, once it is drained
   static_assert(S::kPiece * 4 <= S::kRing, "a piece fits in the ring");
+  constexpr uint32_t kGroupBits = (1u << S::kGroups) - 1u;
   pdl_wait();
   pdl_launch_dependents();
 
@@ -272,7 +305,7 @@ __global__ void __launch_bounds__(kPdThreads, 1) paged_decode_kernel(const Paged
   const int per_thread = (p.c.B + kPdThreads - 1) / kPdThreads;
   const int b_lo = min(p.c.B, tid * per_thread), b_hi = min(p.c.B, b_lo + per_thread);
   long long mine = 0;
-  for (int b = b_lo; b < b_hi; ++b) mine += (long long)tile_span(p, seq_len(p.c, b)).nt * H;
+  for (int b = b_lo; b < b_hi; ++b) mine += (long long)tile_span<S::kTile>(p, seq_len(p.c, b)).nt * H;
   long long incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -303,7 +336,7 @@ __global__ void __launch_bounds__(kPdThreads, 1) paged_decode_kernel(const Paged
       long long excl = mine0;
       int b = b_lo;
       for (; b < b_hi - 1; ++b) {
-        const long long n = (long long)tile_span(p, seq_len(p.c, b)).nt * H;
+        const long long n = (long long)tile_span<S::kTile>(p, seq_len(p.c, b)).nt * H;
         if (at < excl + n) break;
         excl += n;
       }
@@ -317,7 +350,7 @@ __global__ void __launch_bounds__(kPdThreads, 1) paged_decode_kernel(const Paged
   if (r0 < r1) {
     LineCursor cur;
     cur.b = sm_b[warp];
-    cur.span = tile_span(p, seq_len(p.c, cur.b));
+    cur.span = tile_span<S::kTile>(p, seq_len(p.c, cur.b));
     cur.hh = (int)((r0 - sm_first[warp]) / cur.span.nt);
     cur.item0 = sm_first[warp] + (long long)cur.hh * cur.span.nt;
     auto advance = [&](LineCursor& c) {   // to the next item with tiles (one exists while its first tile < total)
@@ -326,20 +359,20 @@ __global__ void __launch_bounds__(kPdThreads, 1) paged_decode_kernel(const Paged
         c.hh = 0;
         do {
           ++c.b;
-          c.span = tile_span(p, seq_len(p.c, c.b));
+          c.span = tile_span<S::kTile>(p, seq_len(p.c, c.b));
         } while (c.span.nt == 0);
       }
     };
     const uint32_t ring = smem_u32(smem) + warp * S::kRing;
     LineCursor ahead = cur;
-    uint32_t lost = 0;   // bit st: the stage's page id was outside the pool, its keys are hidden
+    uint32_t lost = 0;   // kGroups bits per stage: page ids outside the pool
     auto issue = [&](long long tile, int st) {
       if (tile < r1) {
         if (tile >= ahead.item0 + ahead.span.nt) advance(ahead);
-        const int key0 = ahead.span.key0((int)(tile - ahead.item0));
-        const int page = page_id(p.c, ahead.b, key0);
-        lost = page < 0 ? lost | (1u << st) : lost & ~(1u << st);
-        copy_tile<T, HD, ROWS>(p, ahead.span, key0, page, ahead.hh / p.hblocks, ring + st * (2 * S::kTileBytes), lane);
+        const int key0 = tile_key<S::kTile>(ahead.span, (int)(tile - ahead.item0));
+        const uint32_t bad = copy_tile<T, HD, ROWS>(p, ahead.span, ahead.b, key0, ahead.hh / p.hblocks,
+                                                    ring + st * (2 * S::kTileBytes), lane);
+        lost = (lost & ~(kGroupBits << (st * S::kGroups))) | (bad << (st * S::kGroups));
       }
       cp_async_commit();   // one group per call, empty past the run's end
     };
@@ -370,8 +403,8 @@ __global__ void __launch_bounds__(kPdThreads, 1) paged_decode_kernel(const Paged
       for (; tile < end; ++tile) {
         cp_async_wait<S::kStages - 1>();   // the oldest group has landed
         __syncwarp();
-        w.tile(p, cur.span, cur.span.key0((int)(tile - cur.item0)), !((lost >> st) & 1u),
-               ring + st * (2 * S::kTileBytes), lane);
+        w.tile(p, cur.span, tile_key<S::kTile>(cur.span, (int)(tile - cur.item0)),
+               (lost >> (st * S::kGroups)) & kGroupBits, ring + st * (2 * S::kTileBytes), lane);
         __syncwarp();   // every lane has read the stage
         issue(next++, st);
         if (++st == S::kStages) st = 0;
@@ -406,54 +439,68 @@ __global__ void __launch_bounds__(kPdThreads, 1) paged_decode_kernel(const Paged
   }
   __syncthreads();
 
-  // ---- pieces of one item follow one another in the entries
-  int2 open = make_int2(0, 0);
-  for (int e = 0; e < 2 * kPdWarps;) {
-    const int item = sm_item[e];
-    if (item < 0) {
-      ++e;
-      continue;
-    }
-    int end = e + 1;
-    while (end < 2 * kPdWarps && (sm_item[end] < 0 || sm_item[end] == item)) ++end;
-    const int b = sm_b_of[e], hh = item - b * H, kvh = hh / p.hblocks, hb = hh - kvh * p.hblocks;
-    const int rows = min(ROWS, p.group - hb * ROWS);
-    const int more = sm_runs[e];
-    const bool starts = e & 1;
-    if (starts && more) open = make_int2(item, more + 1);
-    float* slot = p.part + (long long)(2 * blockIdx.x + (starts ? 1 : 0)) * S::kPiece;
-    auto piece = [&](int i) {
-      return reinterpret_cast<const float*>(smem + ((i & 1) ? (i >> 1) * S::kRing : kPdWarps * S::kRing +
-                                                                                        (i >> 1) * S::kPiece * 4));
-    };
-    for (int i = tid; i < rows * (HD / 2); i += kPdThreads) {
-      const int r = i / (HD / 2), d = (i - r * (HD / 2)) * 2;
-      float M = -INFINITY;
-      for (int x = e; x < end; ++x)
-        if (sm_item[x] >= 0) M = fmaxf(M, piece(x)[r * S::kStride + HD]);
-      float L = 0.f, x0 = 0.f, x1 = 0.f;
-      for (int x = e; x < end; ++x) {
-        if (sm_item[x] < 0) continue;
-        const float* row = piece(x) + r * S::kStride;
-        const float f = row[HD] == -INFINITY ? 0.f : ex2(row[HD] - M);   // no key seen in this piece
-        const float2 v = *reinterpret_cast<const float2*>(row + d);
-        L = fmaf(row[HD + 1], f, L);
-        x0 = fmaf(v.x, f, x0);
-        x1 = fmaf(v.y, f, x1);
-      }
-      if (starts && !more) {
-        const float inv = L == 0.f ? 0.f : 1.f / L;
-        T* dst = static_cast<T*>(p.out) + b * p.o_b + (long long)(kvh * p.group + hb * ROWS + r) * p.o_h + d;
-        *reinterpret_cast<uint32_t*>(dst) = Elem<T>::pack(x0 * inv, x1 * inv);
-      } else {
-        float* dst = slot + r * S::kStride;
-        *reinterpret_cast<float2*>(dst + d) = make_float2(x0, x1);
-        if (d == 0) *reinterpret_cast<float2*>(dst + HD) = make_float2(M, L);
-      }
-    }
-    e = end;
+  // ---- pieces of one item follow one another in the entries; `firsts` marks the
+  // first of each item's. A warp takes an item's row at a time: lane e has the
+  // weight of entry e, then a lane has HD / 32 dims.
+  const int my_item = lane < 2 * kPdWarps ? sm_item[lane] : -1, my_runs = lane < 2 * kPdWarps ? sm_runs[lane] : 0;
+  const uint32_t valid = __ballot_sync(0xffffffffu, my_item >= 0);
+  uint32_t firsts;
+  {
+    const uint32_t before_me = valid & ((1u << lane) - 1u);
+    const int prev = __shfl_sync(0xffffffffu, my_item, before_me ? 31 - __clz(before_me) : lane);
+    firsts = __ballot_sync(0xffffffffu, my_item >= 0 && (!before_me || prev != my_item));
   }
-  if (tid == 0) p.meta[blockIdx.x] = open;
+  // only the last item can go on in the next CTA; an odd entry: it begins in this one
+  if (tid == 31 - __clz(firsts | 1u))
+    p.meta[blockIdx.x] = (tid & 1) && my_item >= 0 && my_runs ? make_int2(my_item, my_runs + 1) : make_int2(0, 0);
+  auto piece = [&](int e) {   // entry e's first byte
+    return smem_u32(smem) + (uint32_t)((e & 1) ? (e >> 1) * S::kRing : kPdWarps * S::kRing + (e >> 1) * S::kPiece * 4);
+  };
+  constexpr int V = HD / 32;
+  const int rows_max = min(ROWS, p.group), tasks = __popc(firsts) * rows_max;
+  for (int task = warp; task < tasks; task += kPdWarps) {
+    const int k = task / rows_max, r = task - k * rows_max;
+    uint32_t rest = firsts;
+    for (int x = 0; x < k; ++x) rest &= rest - 1u;
+    const int e0 = __ffs(rest) - 1;
+    rest &= rest - 1u;
+    const uint32_t mine = valid & (~0u << e0) & (rest ? (rest & (0u - rest)) - 1u : ~0u);   // the item's entries
+    const int item = __shfl_sync(0xffffffffu, my_item, e0), b = sm_b_of[e0], hh = item - b * H;
+    const int kvh = hh / p.hblocks, hb = hh - kvh * p.hblocks;
+    if (r >= p.group - hb * ROWS) continue;
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if ((mine >> lane) & 1u) ml = lds_f2(piece(lane) + (uint32_t)(r * S::kStride + HD) * 4u);
+    const float M = warp_max(ml.x);
+    const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);   // no key seen in this piece
+    const float L = warp_sum(ml.y * f);
+    float2 acc[V / 2];
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) acc[i] = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int x = 0; x < 2 * kPdWarps; ++x) {
+      if (!((mine >> x) & 1u)) continue;
+      const float g = __shfl_sync(0xffffffffu, f, x);
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) {
+        const float2 v = lds_f2(piece(x) + (uint32_t)(r * S::kStride + lane * V + 2 * i) * 4u);
+        acc[i].x = fmaf(v.x, g, acc[i].x);
+        acc[i].y = fmaf(v.y, g, acc[i].y);
+      }
+    }
+    const bool starts = e0 & 1;
+    if (starts && !__shfl_sync(0xffffffffu, my_runs, e0)) {
+      const float inv = L == 0.f ? 0.f : 1.f / L;
+      T* out = static_cast<T*>(p.out) + b * p.o_b + (long long)(kvh * p.group + hb * ROWS + r) * p.o_h + lane * V;
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i)
+        *reinterpret_cast<uint32_t*>(out + 2 * i) = Elem<T>::pack(acc[i].x * inv, acc[i].y * inv);
+    } else {
+      float* part = p.part + (long long)(2 * blockIdx.x + (starts ? 1 : 0)) * S::kPiece + r * S::kStride;
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) *reinterpret_cast<float2*>(part + lane * V + 2 * i) = acc[i];
+      if (lane == 0) *reinterpret_cast<float2*>(part + HD) = make_float2(M, L);
+    }
+  }
 }
 
 // Joins the pieces of the items that several CTAs hold, in the order of the
@@ -556,15 +603,16 @@ __global__ void __launch_bounds__(kPdThreads, 1) paged_decode_cluster_kernel(con
   pdl_launch_dependents();
   Item w;
   Item::load_q(p, b, head0, rows, lane, w.qa);
-  const TileSpan sp = tile_span(p, seq_len(p.c, b));
+  const TileSpan sp = tile_span<S::kTile>(p, seq_len(p.c, b));
+  constexpr uint32_t kGroupBits = (1u << S::kGroups) - 1u;
   const int step = CL * kPdWarps;
   const uint32_t ring = smem_u32(smem) + warp * S::kRing;
   uint32_t lost = 0;
   auto issue = [&](int tile, int st) {
     if (tile < sp.nt) {
-      const int key0 = sp.key0(tile), page = page_id(p.c, b, key0);
-      lost = page < 0 ? lost | (1u << st) : lost & ~(1u << st);
-      copy_tile<T, HD, ROWS>(p, sp, key0, page, kvh, ring + st * (2 * S::kTileBytes), lane);
+      const uint32_t bad =
+          copy_tile<T, HD, ROWS>(p, sp, b, tile_key<S::kTile>(sp, tile), kvh, ring + st * (2 * S::kTileBytes), lane);
+      lost = (lost & ~(kGroupBits << (st * S::kGroups))) | (bad << (st * S::kGroups));
     }
     cp_async_commit();
   };
@@ -575,7 +623,8 @@ __global__ void __launch_bounds__(kPdThreads, 1) paged_decode_cluster_kernel(con
   for (; tile < sp.nt; tile += step) {
     cp_async_wait<S::kStages - 1>();
     __syncwarp();
-    w.tile(p, sp, sp.key0(tile), !((lost >> st) & 1u), ring + st * (2 * S::kTileBytes), lane);
+    w.tile(p, sp, tile_key<S::kTile>(sp, tile), (lost >> (st * S::kGroups)) & kGroupBits,
+           ring + st * (2 * S::kTileBytes), lane);
     __syncwarp();
     issue(next, st);
     next += step;
@@ -652,20 +701,15 @@ DecodePlan decode_plan(const lw_paged_attention_args* a) {
   d.items = (long long)a->cache.batch * a->cache.n_kv_heads * d.hblocks;
   d.grid = lw_host::sm_count();
   // Clusters of as many CTAs as the SMs hold beside each other (up to 8), when
-  // no sequence can give one of their CTAs more than 32 tiles (four per warp).
+  // no sequence can give one of their CTAs more than 512 keys (a few tiles per warp).
   long long keys = (long long)a->cache.table_width * a->cache.page_size;
   if (a->window > 0) keys = std::min(keys, (long long)a->window + a->sinks);
   d.cluster = 8;
   while (d.cluster > 1 && d.items * d.cluster > d.grid) d.cluster /= 2;
-  if (d.items * d.cluster > d.grid || keys > 32ll * lw::kPdTile * d.cluster) d.cluster = 0;
+  if (d.items * d.cluster > d.grid || keys > 512ll * d.cluster) d.cluster = 0;
   d.part_off = ((size_t)d.grid * sizeof(int2) + 255) & ~(size_t)255;
   d.bytes = d.cluster ? 0 : d.part_off + (size_t)2 * d.grid * d.rows * (a->cache.head_dim + 8) * sizeof(float);
   return d;
-}
-
-template <typename Kernel>
-cudaError_t allow_smem(Kernel kern, int bytes) {
-  return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 
 template <typename T, int HD, int ROWS>
@@ -673,7 +717,7 @@ cudaError_t decode_launch(const lw::PagedDecodeParams& p, const DecodePlan& d, c
   constexpr int smem = lw::DecodeShape<HD, ROWS>::kBytes;
   if (d.cluster) {
     auto kern = lw::paged_decode_cluster_kernel<T, HD, ROWS>;
-    cudaError_t e = allow_smem(kern, smem);
+    cudaError_t e = lw_host::allow_smem<lw::paged_decode_cluster_kernel<T, HD, ROWS>>(smem);
     if (e != cudaSuccess) return e;
     lw_count_launch();
     cudaLaunchConfig_t cfg = {};
@@ -693,7 +737,7 @@ cudaError_t decode_launch(const lw::PagedDecodeParams& p, const DecodePlan& d, c
     return cudaLaunchKernelEx(&cfg, kern, p);
   }
   auto kern = lw::paged_decode_kernel<T, HD, ROWS>;
-  cudaError_t e = allow_smem(kern, smem);
+  cudaError_t e = lw_host::allow_smem<lw::paged_decode_kernel<T, HD, ROWS>>(smem);
   if (e != cudaSuccess) return e;
   e = lw_launch(kern, dim3(d.grid), dim3(lw::kPdThreads), smem, s, pdl, p);
   if (e != cudaSuccess) return e;

@@ -762,7 +762,7 @@ template <typename T, int HD>
 cudaError_t prompt_launch(const lw::PromptParams& p, cudaStream_t s, bool pdl) {
   constexpr int smem = lw::PromptSmem<HD>::kBytes;
   auto kern = lw::paged_prompt_kernel<T, HD>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = lw_host::allow_smem<lw::paged_prompt_kernel<T, HD>>(smem);
   if (e != cudaSuccess) return e;
   e = lw_launch(kern, dim3((unsigned)(p.T / (2 * p.rp) + p.c.B), (unsigned)p.c.nkv, (unsigned)p.slices),
                 dim3(lw::kPmThreads), smem, s, pdl, p);
