@@ -37,6 +37,9 @@ from liteweight_b200 import _native as nat
 c_int, c_void_p, c_float, c_size_t, c_ll = (ctypes.c_int, ctypes.c_void_p, ctypes.c_float, ctypes.c_size_t,
                                             ctypes.c_longlong)
 _INT_MAX = 2**31 - 1
+_WORKSPACE = 7   # LW_ERR_WORKSPACE
+# what torch.cuda.current_device() and current_stream().cuda_stream come to
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 _F16, _BF16, _F32, _I32 = torch.float16, torch.bfloat16, torch.float32, torch.int32
 
 
@@ -82,10 +85,10 @@ nat.register("lw_paged_attention_workspace_size", [c_void_p], c_size_t)
 def _rows(name: str, t: torch.Tensor, dtype: torch.dtype, hd: int) -> tuple[int, int]:
     """(token, head) strides of a [tokens, heads, head_dim] tensor."""
     assert t.dtype is dtype, f"{name} is {t.dtype}, the cache {dtype}"
-    assert t.dim() == 3 and t.shape[2] == hd, f"{name} must be [tokens, heads, {hd}], got {tuple(t.shape)}"
-    st, sh, sd = t.stride()
-    assert sd == 1 or t.numel() == 0, f"{name}'s last dimension must be contiguous"
-    return st, sh
+    strides = t.stride()
+    assert len(strides) == 3 and t.shape[2] == hd, f"{name} must be [tokens, heads, {hd}], got {tuple(t.shape)}"
+    assert strides[2] == 1 or t.numel() == 0, f"{name}'s last dimension must be contiguous"
+    return strides[:2]
 
 
 def _cache_fields(k_pages, v_pages, page_table, kv_lens) -> tuple:
@@ -94,9 +97,10 @@ def _cache_fields(k_pages, v_pages, page_table, kv_lens) -> tuple:
     shape = k_pages.shape
     assert len(shape) == 4 and shape == v_pages.shape, "k_pages / v_pages: [pages, kv heads, page, head_dim]"
     assert page_table.dtype is _I32 and kv_lens.dtype is _I32, "page_table and kv_lens are int32"
-    ks, vs, ts, tshape = k_pages.stride(), v_pages.stride(), page_table.stride(), page_table.shape
-    assert len(tshape) == 2 and kv_lens.shape == tshape[:1], "page_table: [batch, width], kv_lens: [batch]"
-    batch, width = tshape
+    ks, vs, ts = k_pages.stride(), v_pages.stride(), page_table.stride()
+    assert len(ts) == 2 and kv_lens.dim() == 1, "page_table: [batch, width], kv_lens: [batch]"
+    batch, width = page_table.shape
+    assert len(kv_lens) == batch, "page_table: [batch, width], kv_lens: [batch]"
     assert (ks[3] == 1 and vs[3] == 1) or k_pages.numel() == 0, "the pools' last dimension must be contiguous"
     assert ts[1] == 1 or width <= 1, "page_table's rows must be contiguous"
     assert batch <= 1 or kv_lens.stride(0) == 1, "kv_lens must be contiguous"
@@ -113,24 +117,23 @@ def _offsets(q_offsets, batch: int, tokens: int) -> int:
     return q_offsets.data_ptr()
 
 
-def _device_of(*ts) -> int:
-    """Index of the one device that holds them all."""
-    dev = ts[0].get_device()
-    for t in ts:
-        if t is not None and (dev < 0 or t.get_device() != dev):
-            nat.require_cuda(*ts)
-            raise AssertionError("all tensors must be on one device")
-    return dev
+def _refuse_devices(*ts) -> None:
+    nat.require_cuda(*ts)
+    raise AssertionError("all tensors must be on one device")
 
 
 def _run(fn: str, args: bytes, dev: int) -> None:
-    if torch.cuda.current_device() == dev:
-        status = getattr(nat.lib(), fn)(args, torch._C._cuda_getCurrentRawStream(dev))
-    else:
-        with torch.cuda.device(dev):
-            status = getattr(nat.lib(), fn)(args, torch._C._cuda_getCurrentRawStream(dev))
+    status = _status(getattr(nat.lib(), fn), args, dev)
     if status:
         nat.check(fn, status)
+
+
+def _status(call, args: bytes, dev: int) -> int:
+    """One C call on the current stream of device `dev`, as the current device."""
+    if _current_device() == dev:
+        return call(args, _raw_stream(dev))
+    with torch.cuda.device(dev):
+        return call(args, _raw_stream(dev))
 
 
 def check_device_error() -> None:
@@ -180,13 +183,15 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.T
             assert w.dtype is dt and w.shape == (hd,) and w.stride(0) == 1, f"norm weights: {dt} [{hd}]"
     off = _offsets(q_offsets, batch, T)
     assert out is None or out.shape == q.shape, "out must have q's shape"
-    dev = _device_of(q, k, v, cos, sin, k_pages, v_pages, page_table, kv_lens, q_offsets, q_weight, k_weight, out)
+    dev = q.get_device()
+    if not (0 <= dev == k.get_device() == v.get_device() == cos.get_device() == sin.get_device() == k_pages.get_device()
+            == v_pages.get_device() == page_table.get_device() == kv_lens.get_device()
+            and all(t is None or t.get_device() == dev for t in (q_offsets, q_weight, k_weight, out))):
+        _refuse_devices(q, k, v, cos, sin, k_pages, v_pages, page_table, kv_lens, q_offsets, q_weight, k_weight, out)
     fresh = out is None
     if fresh:
-        out = torch.empty((T, nq, hd), dtype=dt, device=q.device)
-        os_ = (nq * hd, hd)
-    else:
-        os_ = _rows("out", out, dt, hd)
+        out = torch.empty_like(q)
+    os_ = _rows("out", out, dt, hd)
     _run("lw_qk_norm_rope", _ROPE.pack(
         *cache, q.data_ptr(), k.data_ptr(), v.data_ptr(), *qs, *ks, *vs, out.data_ptr(), *os_, T, nq, off,
         cos.data_ptr(), sin.data_ptr(), ts[0], 2 if tt is _F32 else cache[12], tshape[0],
@@ -205,21 +210,24 @@ def _attention(q, k_pages, v_pages, page_table, kv_lens, q_offsets, window, sink
     assert sinks >= 0, "sinks: at least 0"
     off = _offsets(q_offsets, batch, T)
     assert out is None or (out.shape == q.shape and out.dtype is dt), "out must have q's shape and type"
-    dev = _device_of(q, k_pages, v_pages, page_table, kv_lens, q_offsets, out)
+    dev = q.get_device()
+    if not (0 <= dev == k_pages.get_device() == v_pages.get_device() == page_table.get_device() == kv_lens.get_device()
+            and (q_offsets is None or q_offsets.get_device() == dev) and (out is None or out.get_device() == dev)):
+        _refuse_devices(q, k_pages, v_pages, page_table, kv_lens, q_offsets, out)
     fresh = out is None
     if fresh:
-        out = torch.empty((T, nq, hd), dtype=dt, device=q.device)
-        os_ = (nq * hd, hd)
-    else:
-        os_ = _rows("out", out, dt, hd)
-    fields = (*cache, q.data_ptr(), *qs, out.data_ptr(), *os_, T, nq, off, min(window or 0, _INT_MAX),
-              min(sinks, _INT_MAX), hd ** -0.5 if scale is None else scale, fresh, 1)
-    args = _ATTN.pack(*fields, 0, 0)
-    need = nat.lib().lw_paged_attention_workspace_size(args)
-    if need:   # scratch of this call alone: calls on other streams or in other graphs never share it
+        out = torch.empty_like(q)
+    fields = (*cache, q.data_ptr(), *qs, out.data_ptr(), *_rows("out", out, dt, hd), T, nq, off,
+              min(window or 0, _INT_MAX), min(sinks, _INT_MAX), hd ** -0.5 if scale is None else scale, fresh, 1)
+    lib, args = nat.lib(), _ATTN.pack(*fields, 0, 0)
+    status = _status(lib.lw_paged_attention, args, dev)
+    if status == _WORKSPACE:   # not a short one: with scratch of this call alone, which no other stream or graph shares
+        with torch.cuda.device(dev):
+            need = lib.lw_paged_attention_workspace_size(args)
         ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-        args = _ATTN.pack(*fields, ws.data_ptr(), need)
-    _run("lw_paged_attention", args, dev)
+        status = _status(lib.lw_paged_attention, _ATTN.pack(*fields, ws.data_ptr(), ws.numel()), dev)
+    if status:
+        nat.check("lw_paged_attention", status)
     return out
 
 
