@@ -86,7 +86,6 @@ struct PromptWork {
   int kvh, slice, b;
   int tok0, np;        // first row of q, positions
   int pos0, last;      // position of the first, of the last
-  int len;
   int lo0;             // first key that the window of any row reaches
   int ns, w0, t0, nt;  // tiles 0 .. ns - 1 and w0 .. are seen; the slice is the nt from the t0-th on
   LW_DEV int key_of(int i) const { return (t0 + i < ns ? t0 + i : w0 + t0 + i - ns) * kPmKeys; }
@@ -117,20 +116,23 @@ LW_DEV bool find_work(const PromptParams& p, int slot, int kvh, int slice, Promp
     hi = min(hi, lo + step);
   }
   const int i0 = (slot - (o / R + lo)) * R;
-  if (!(i0 >= 0 && i0 < n && o >= 0 && (long long)o + n <= p.T)) return false;
+  if (i0 < 0 || i0 >= n) return false;
+  if (o < 0 || (long long)o + n > p.T) {   // rows that q does not have
+    lw_record_error(LW_ERR_BAD_INDEX);
+    return false;
+  }
   w.valid = 1;
   w.kvh = kvh;
   w.slice = slice;
   w.b = lo;
   w.tok0 = o + i0;
   w.np = min(R, n - i0);
-  w.len = cut_len(p.c, len);
-  w.pos0 = len - n + i0;   // negative: more rows than tokens
+  w.pos0 = cut_len(p.c, len) - n + i0;   // negative: more rows than tokens
   if (w.pos0 < 0) lw_record_error(LW_ERR_BAD_INDEX);
-  w.last = min(w.pos0 + w.np, w.len) - 1;
+  w.last = w.pos0 + w.np - 1;
   w.lo0 = window_start(max(w.pos0, 0), p.window);
   w.w0 = w.lo0 / kPmKeys;
-  w.ns = p.window > 0 ? min((p.sinks + kPmKeys - 1) / kPmKeys, w.w0) : 0;
+  w.ns = p.window > 0 ? min((min(p.sinks, w.lo0) + kPmKeys - 1) / kPmKeys, w.w0) : 0;
   const int all = w.last < 0 ? 0 : w.ns + w.last / kPmKeys + 1 - w.w0;
   w.t0 = (int)((long long)all * slice / p.slices);
   w.nt = (int)((long long)all * (slice + 1) / p.slices) - w.t0;
@@ -466,11 +468,14 @@ __global__ void __launch_bounds__(kPmThreads, 1) paged_prompt_kernel(const __gri
         if (!warp_wait(smem_u32(&bar_clc), asked++ & 1)) break;
         more = clc_answer(smem_u32(&clc_s), x, y, z);
         __syncwarp();
-        if (p.zero_tail && slice == 0) {   // rows of no sequence
-          for (int r = max(0, p.off[p.c.B]) + slot; r < p.T; r += slots)
+        if (p.zero_tail && slice == 0) {   // rows of no sequence: before the first, behind the last
+          const int first = max(0, min(p.T, p.off[0])), behind = max(first, p.off[p.c.B]);
+          for (int x0 = slot; x0 < first + max(0, p.T - behind); x0 += slots) {
+            const int r = x0 < first ? x0 : behind + x0 - first;
             for (int i = lane; i < p.group * (HD / 8); i += 32)
               *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + r * p.o_t + (kvh * p.group + i / (HD / 8)) * p.o_h +
                                         (i % (HD / 8)) * 8) = make_uint4(0, 0, 0, 0);
+          }
         }
       }
       w.valid = 0;
@@ -494,8 +499,8 @@ __global__ void __launch_bounds__(kPmThreads, 1) paged_prompt_kernel(const __gri
       }
       const int npos = min(p.rp, w.np - g * p.rp);
       const bool have = r < npos * p.group;
-      const int first_pos = w.pos0 + g * p.rp, last_pos = min(first_pos + npos, w.len) - 1;
-      const int pos = have ? min(first_pos + r_pos, w.len - 1) : -1;
+      const int first_pos = w.pos0 + g * p.rp, last_pos = first_pos + npos - 1;
+      const int pos = have ? first_pos + r_pos : -1;
       const int lo = windowed ? pos - p.window : -1;   // keys above lo, or below sinks
       const int sinks = windowed ? p.sinks : 0;
       float m = -INFINITY, l = 0.f;

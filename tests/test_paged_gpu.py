@@ -200,6 +200,54 @@ def test_bad_indexes_are_skipped_and_recorded():
         kernels.check_device_error()
 
 
+@pytest.mark.parametrize("window,sinks", [(None, 0), (20, 0), (20, 5)])
+def test_lengths_past_the_table_are_cut(window, sinks):
+    """The chunk's rows are then the last the table addresses."""
+    from liteweight_b200._native import LiteweightError
+    c = Batch([64], 1, 64, 16, torch.float16)
+    c.table = c.table[:, :4].contiguous()
+    q = torch.randn(30, 2, 64, generator=gen(2), device=DEV).half()
+    off = torch.tensor([0, 30], dtype=torch.int32, device=DEV)
+    for length in (90, 10 ** 9, 2 ** 31 - 1):
+        c.kv_lens[0] = length
+        got = kernels.prompt_attention(q, *c.cache(), off, window=window, sinks=sinks)
+        with pytest.raises(LiteweightError, match="out of range"):
+            kernels.check_device_error()
+        check(got, *attend(q, c.k[0], c.v[0], 34, window, sinks, 0.125, torch.float16))
+        got = kernels.paged_attention(q[:1], *c.cache(), window=window, sinks=sinks)
+        with pytest.raises(LiteweightError, match="out of range"):
+            kernels.check_device_error()
+        check(got, *attend(q[:1], c.k[0], c.v[0], 63, window, sinks, 0.125, torch.float16))
+
+
+def test_offsets_past_the_rows_are_refused_on_the_device():
+    from liteweight_b200._native import LiteweightError
+    c = Batch([40, 30], 1, 64, 16, torch.float16)
+    q = torch.randn(20, 2, 64, generator=gen(2), device=DEV).half()
+    off = torch.tensor([0, 12, 25], dtype=torch.int32, device=DEV)   # rows 20 .. 24 are not there
+    got = kernels.prompt_attention(q, *c.cache(), off)
+    with pytest.raises(LiteweightError, match="out of range"):
+        kernels.check_device_error()
+    check(got[:12], *attend(q[:12], c.k[0], c.v[0], 28, None, 0, 0.125, torch.float16))
+    off = torch.tensor([3, 12, 18], dtype=torch.int32, device=DEV)   # rows before the first and behind the last
+    got = kernels.prompt_attention(q, *c.cache(), off)
+    kernels.check_device_error()
+    assert (got[:3] == 0).all() and (got[18:] == 0).all()
+    check(got[3:12], *attend(q[3:12], c.k[0], c.v[0], 31, None, 0, 0.125, torch.float16))
+
+
+def test_largest_windows_and_sinks():
+    c = Batch([300, 20], 2, 64, 16, torch.float16)
+    q = torch.randn(2, 4, 64, generator=gen(2), device=DEV).half()
+    off = torch.tensor([0, 1, 2], dtype=torch.int32, device=DEV)
+    want, cut = kernels.paged_attention(q, *c.cache()), kernels.paged_attention(q, *c.cache(), window=7, sinks=2)
+    for window, sinks, x in ((2 ** 40, 0, want), (2 ** 31 - 1, 2 ** 40, want), (1, 2 ** 31 - 1, want), (7, 2, cut)):
+        for got in (kernels.paged_attention(q, *c.cache(), window=window, sinks=sinks),
+                    kernels.prompt_attention(q, *c.cache(), off, window=window, sinks=sinks)):
+            assert (got.float() - x.float()).abs().max() < 4e-3
+    kernels.check_device_error()
+
+
 def test_far_pages():
     """Offsets past 2^31 elements: a pool of 5 GB of which the last pages are used."""
     nkv, page, hd = 8, 256, 128
