@@ -8,6 +8,8 @@ or fails to load, every op raises.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import threading
 from pathlib import Path
@@ -15,8 +17,10 @@ from pathlib import Path
 import torch
 
 _LIB_PATH = Path(__file__).resolve().parent / "_lib" / "liblw_b200.so"
+_BIND_PATH = _LIB_PATH.with_name("lw_bind.so")
 _lock = threading.Lock()
 _lib = None
+_bind = None
 
 c_int, c_void_p = ctypes.c_int, ctypes.c_void_p
 
@@ -87,6 +91,25 @@ def lib() -> ctypes.CDLL:
                 fn.restype = _RESTYPE.get(name, c_int)
             _lib = handle
     return _lib
+
+
+def bind():
+    """The extension module over the paged-cache entry points (csrc/bind_paged.cpp),
+    loaded once; its calls go to lib()'s functions."""
+    global _bind
+    if _bind is None:
+        handle = lib()
+        if not _BIND_PATH.exists():
+            raise RuntimeError(f"liteweight_b200 extension module not found at {_BIND_PATH}; build it with "
+                               "`python -m liteweight_b200.build`")
+        loader = importlib.machinery.ExtensionFileLoader("lw_bind", str(_BIND_PATH))
+        module = importlib.util.module_from_spec(importlib.util.spec_from_file_location("lw_bind", _BIND_PATH,
+                                                                                       loader=loader))
+        loader.exec_module(module)
+        module.init(*(ctypes.cast(getattr(handle, f), c_void_p).value for f in
+                      ("lw_qk_norm_rope", "lw_paged_attention", "lw_paged_attention_workspace_size")))
+        _bind = module
+    return _bind
 
 
 def check(fn: str, status: int) -> None:

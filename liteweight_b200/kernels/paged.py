@@ -28,7 +28,6 @@ output and scratch from torch, and can be captured in a CUDA graph.
 from __future__ import annotations
 
 import ctypes
-import struct
 
 import torch
 
@@ -36,11 +35,6 @@ from liteweight_b200 import _native as nat
 
 c_int, c_void_p, c_float, c_size_t, c_ll = (ctypes.c_int, ctypes.c_void_p, ctypes.c_float, ctypes.c_size_t,
                                             ctypes.c_longlong)
-_INT_MAX = 2**31 - 1
-_WORKSPACE = 7   # LW_ERR_WORKSPACE
-# what torch.cuda.current_device() and current_stream().cuda_stream come to
-_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
-_F16, _BF16, _F32, _I32 = torch.float16, torch.bfloat16, torch.float32, torch.int32
 
 
 class PagedCacheArgs(ctypes.Structure):
@@ -69,71 +63,9 @@ class PagedAttentionArgs(ctypes.Structure):
                 ("workspace", c_void_p), ("workspace_bytes", c_size_t)]
 
 
-# The calls below write the same structs with struct.pack (one call instead of a
-# ctypes object per field: a decode step makes two of them per layer). Native
-# alignment, so the layouts are the C compiler's.
-_CACHE_FMT = "PP6q6iPqi0qP"
-_ROPE = struct.Struct("@" + _CACHE_FMT + "PPP6qP2qii0qPPPqiiPPfii0q")
-_ATTN = struct.Struct("@" + _CACHE_FMT + "P2qP2qii0qPiifii0qPN")
-assert _ROPE.size == ctypes.sizeof(QkNormRopeArgs) and _ATTN.size == ctypes.sizeof(PagedAttentionArgs)
-
-nat.register("lw_qk_norm_rope", [c_void_p, c_void_p])
-nat.register("lw_paged_attention", [c_void_p, c_void_p])
-nat.register("lw_paged_attention_workspace_size", [c_void_p], c_size_t)
-
-
-def _rows(name: str, t: torch.Tensor, dtype: torch.dtype, hd: int) -> tuple[int, int]:
-    """(token, head) strides of a [tokens, heads, head_dim] tensor."""
-    assert t.dtype is dtype, f"{name} is {t.dtype}, the cache {dtype}"
-    strides = t.stride()
-    assert len(strides) == 3 and t.shape[2] == hd, f"{name} must be [tokens, heads, {hd}], got {tuple(t.shape)}"
-    assert strides[2] == 1 or t.numel() == 0, f"{name}'s last dimension must be contiguous"
-    return strides[:2]
-
-
-def _cache_fields(k_pages, v_pages, page_table, kv_lens) -> tuple:
-    dt = k_pages.dtype
-    assert (dt is _F16 or dt is _BF16) and v_pages.dtype is dt, "k_pages / v_pages: both float16 or both bfloat16"
-    shape = k_pages.shape
-    assert len(shape) == 4 and shape == v_pages.shape, "k_pages / v_pages: [pages, kv heads, page, head_dim]"
-    assert page_table.dtype is _I32 and kv_lens.dtype is _I32, "page_table and kv_lens are int32"
-    ks, vs, ts = k_pages.stride(), v_pages.stride(), page_table.stride()
-    assert len(ts) == 2 and kv_lens.dim() == 1, "page_table: [batch, width], kv_lens: [batch]"
-    batch, width = page_table.shape
-    assert len(kv_lens) == batch, "page_table: [batch, width], kv_lens: [batch]"
-    assert (ks[3] == 1 and vs[3] == 1) or k_pages.numel() == 0, "the pools' last dimension must be contiguous"
-    assert ts[1] == 1 or width <= 1, "page_table's rows must be contiguous"
-    assert batch <= 1 or kv_lens.stride(0) == 1, "kv_lens must be contiguous"
-    return (k_pages.data_ptr(), v_pages.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], shape[0], shape[2],
-            shape[1], shape[3], 0 if dt is _F16 else 1, batch, page_table.data_ptr(), ts[0], width, kv_lens.data_ptr())
-
-
-def _offsets(q_offsets, batch: int, tokens: int) -> int:
-    if q_offsets is None:
-        assert tokens == batch, f"one new token per sequence: {tokens} rows for {batch} sequences"
-        return 0
-    assert q_offsets.dtype is _I32 and q_offsets.shape == (batch + 1,), f"q_offsets: int32 [{batch + 1}]"
-    assert q_offsets.stride(0) == 1, "q_offsets must be contiguous"
-    return q_offsets.data_ptr()
-
-
-def _refuse_devices(*ts) -> None:
-    nat.require_cuda(*ts)
-    raise AssertionError("all tensors must be on one device")
-
-
-def _run(fn: str, args: bytes, dev: int) -> None:
-    status = _status(getattr(nat.lib(), fn), args, dev)
-    if status:
-        nat.check(fn, status)
-
-
-def _status(call, args: bytes, dev: int) -> int:
-    """One C call on the current stream of device `dev`, as the current device."""
-    if _current_device() == dev:
-        return call(args, _raw_stream(dev))
-    with torch.cuda.device(dev):
-        return call(args, _raw_stream(dev))
+nat.register("lw_qk_norm_rope", [ctypes.POINTER(QkNormRopeArgs), c_void_p])
+nat.register("lw_paged_attention", [ctypes.POINTER(PagedAttentionArgs), c_void_p])
+nat.register("lw_paged_attention_workspace_size", [ctypes.POINTER(PagedAttentionArgs)], c_size_t)
 
 
 def check_device_error() -> None:
@@ -168,67 +100,18 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.T
     q_offsets[-1] on) are zero, or left as they were in a given `out`. New tokens
     must not share a slot.
     """
-    cache = _cache_fields(k_pages, v_pages, page_table, kv_lens)
-    dt, nkv, hd, batch = k_pages.dtype, cache[10], cache[11], cache[13]
-    qs, ks, vs = _rows("q", q, dt, hd), _rows("k", k, dt, hd), _rows("v", v, dt, hd)
-    T, nq, _ = q.shape
-    assert k.shape == (T, nkv, hd) and v.shape == k.shape, f"k and v: [{T}, {nkv}, {hd}]"
-    tt, tshape, ts = cos.dtype, cos.shape, cos.stride()
-    assert len(tshape) == 2 and tshape[1] == hd and tshape == sin.shape, f"cos / sin: [positions, {hd}]"
-    assert (tt is dt or tt is _F32) and sin.dtype is tt, f"cos / sin: {dt} or float32"
-    assert ts == sin.stride() and (ts[1] == 1 or cos.numel() == 0), "cos / sin: rows contiguous, strides alike"
-    assert (q_weight is None) == (k_weight is None), "norm weights for both queries and keys, or for neither"
-    if q_weight is not None:
-        for w in (q_weight, k_weight):
-            assert w.dtype is dt and w.shape == (hd,) and w.stride(0) == 1, f"norm weights: {dt} [{hd}]"
-    off = _offsets(q_offsets, batch, T)
-    assert out is None or out.shape == q.shape, "out must have q's shape"
-    dev = q.get_device()
-    if not (0 <= dev == k.get_device() == v.get_device() == cos.get_device() == sin.get_device() == k_pages.get_device()
-            == v_pages.get_device() == page_table.get_device() == kv_lens.get_device()
-            and all(t is None or t.get_device() == dev for t in (q_offsets, q_weight, k_weight, out))):
-        _refuse_devices(q, k, v, cos, sin, k_pages, v_pages, page_table, kv_lens, q_offsets, q_weight, k_weight, out)
-    fresh = out is None
-    if fresh:
-        out = torch.empty_like(q)
-    os_ = _rows("out", out, dt, hd)
-    _run("lw_qk_norm_rope", _ROPE.pack(
-        *cache, q.data_ptr(), k.data_ptr(), v.data_ptr(), *qs, *ks, *vs, out.data_ptr(), *os_, T, nq, off,
-        cos.data_ptr(), sin.data_ptr(), ts[0], 2 if tt is _F32 else cache[12], tshape[0],
-        0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(), eps, fresh, 1),
-        dev)
-    return out
+    got = nat.bind().qk_norm_rope(q, k, v, cos, sin, k_pages, v_pages, page_table, kv_lens, q_offsets, q_weight, k_weight,
+                                  eps, out)
+    if type(got) is int:
+        nat.check("lw_qk_norm_rope", got)
+    return got
 
 
 def _attention(q, k_pages, v_pages, page_table, kv_lens, q_offsets, window, sinks, scale, out):
-    cache = _cache_fields(k_pages, v_pages, page_table, kv_lens)
-    dt, hd, batch = k_pages.dtype, cache[11], cache[13]
-    qs = _rows("q", q, dt, hd)
-    T, nq, _ = q.shape
-    assert nq % cache[10] == 0, f"{nq} query heads over {cache[10]} kv heads"
-    assert window is None or window >= 1, "window: at least 1, or None"
-    assert sinks >= 0, "sinks: at least 0"
-    off = _offsets(q_offsets, batch, T)
-    assert out is None or (out.shape == q.shape and out.dtype is dt), "out must have q's shape and type"
-    dev = q.get_device()
-    if not (0 <= dev == k_pages.get_device() == v_pages.get_device() == page_table.get_device() == kv_lens.get_device()
-            and (q_offsets is None or q_offsets.get_device() == dev) and (out is None or out.get_device() == dev)):
-        _refuse_devices(q, k_pages, v_pages, page_table, kv_lens, q_offsets, out)
-    fresh = out is None
-    if fresh:
-        out = torch.empty_like(q)
-    fields = (*cache, q.data_ptr(), *qs, out.data_ptr(), *_rows("out", out, dt, hd), T, nq, off,
-              min(window or 0, _INT_MAX), min(sinks, _INT_MAX), hd ** -0.5 if scale is None else scale, fresh, 1)
-    lib, args = nat.lib(), _ATTN.pack(*fields, 0, 0)
-    status = _status(lib.lw_paged_attention, args, dev)
-    if status == _WORKSPACE:   # not a short one: with scratch of this call alone, which no other stream or graph shares
-        with torch.cuda.device(dev):
-            need = lib.lw_paged_attention_workspace_size(args)
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-        status = _status(lib.lw_paged_attention, _ATTN.pack(*fields, ws.data_ptr(), ws.numel()), dev)
-    if status:
-        nat.check("lw_paged_attention", status)
-    return out
+    got = nat.bind().attention(q, k_pages, v_pages, page_table, kv_lens, q_offsets, window, sinks, scale, out)
+    if type(got) is int:
+        nat.check("lw_paged_attention", got)
+    return got
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
