@@ -693,20 +693,56 @@ struct DecodePlan {
   size_t part_off, bytes;
 };
 
+// Clusters of `size` CTAs with a kernel's shared memory that run at once on the current device.
+int resident_clusters(int size) {
+  static std::atomic<int> known[64][4];   // by device and size, 0: not asked yet
+  int dev = 0, log = 0, n = 0;
+  while ((1 << log) < size) ++log;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  if ((n = known[dev][log].load(std::memory_order_relaxed)) != 0) return std::max(n, 0);
+  constexpr auto kern = lw::paged_decode_cluster_kernel<__half, 128, 8>;
+  constexpr int smem = lw::DecodeShape<128, 8>::kBytes;   // the largest of all forms
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)size;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)size, 148);
+  cfg.blockDim = dim3(lw::kPdThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (lw_host::allow_smem<kern>(smem) != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) {
+    cudaGetLastError();   // no device: no clusters
+    return 0;
+  }
+  known[dev][log].store(n > 0 ? n : -1, std::memory_order_relaxed);
+  return n;
+}
+
 DecodePlan decode_plan(const lw_paged_attention_args* a) {
   DecodePlan d;
   d.group = a->n_q_heads / a->cache.n_kv_heads;
   d.rows = d.group <= 8 ? 8 : 16;
   d.hblocks = (d.group + d.rows - 1) / d.rows;
   d.items = (long long)a->cache.batch * a->cache.n_kv_heads * d.hblocks;
-  d.grid = lw_host::sm_count();
-  // Clusters of as many CTAs as the SMs hold beside each other (up to 8), when
-  // no sequence can give one of their CTAs more than 512 keys (a few tiles per warp).
+  // Runs: 128 CTAs on the 148 SMs. With one on every SM the CTAs of some groups of
+  // neighbouring SMs end 10 to 20 % after the others; with an SM in eight idle they
+  // end together, and the memory is as busy. 128 against 148 CTAs, us: one sequence
+  // of 131071 keys 85.7 / 91.9, 64 ragged ones of up to 16384 145.0 / 152.9, 64 of 2048
+  // 86.6 / 95.9, 32 of 4096 (head_dim 64) 48.6 / 52.5, 160 under a window of 1024 67.4 / 66.8.
+  const int sms = lw_host::sm_count();
+  d.grid = sms >= 32 ? sms / 32 * 32 : sms;
+  // Clusters: the largest of 8, 4, 2 or 1 CTAs of which one per item runs at once,
+  // when no sequence can give a CTA more than 1024 keys, or 512 where the items
+  // fill less than 64 SMs (the runs then use more of them). Cluster / runs, us: 8 items of 2048 keys
+  // 6.7 / 9.5, of 8192 14.4 / 15.3, of 16384 22.8 / 19.6; 1 item of 4096 8.9 / 10.0,
+  // of 8192 13.4 / 10.7; 32 items of 4096 15.9 / 19.9; 128 items of 512 9.2 / 14.6.
   long long keys = (long long)a->cache.table_width * a->cache.page_size;
   if (a->window > 0) keys = std::min(keys, (long long)a->window + a->sinks);
   d.cluster = 8;
-  while (d.cluster > 1 && d.items * d.cluster > d.grid) d.cluster /= 2;
-  if (d.items * d.cluster > d.grid || keys > 512ll * d.cluster) d.cluster = 0;
+  while (d.cluster > 0 && d.items > resident_clusters(d.cluster)) d.cluster /= 2;
+  if (keys > (d.items * d.cluster >= 64 ? 1024ll : 512ll) * d.cluster) d.cluster = 0;
   d.part_off = ((size_t)d.grid * sizeof(int2) + 255) & ~(size_t)255;
   d.bytes = d.cluster ? 0 : d.part_off + (size_t)2 * d.grid * d.rows * (a->cache.head_dim + 8) * sizeof(float);
   return d;
