@@ -726,13 +726,10 @@ DecodePlan decode_plan(const lw_paged_attention_args* a) {
   d.rows = d.group <= 8 ? 8 : 16;
   d.hblocks = (d.group + d.rows - 1) / d.rows;
   d.items = (long long)a->cache.batch * a->cache.n_kv_heads * d.hblocks;
-  // Runs: 128 CTAs on the 148 SMs. With one on every SM the CTAs of some groups of
-  // neighbouring SMs end 10 to 20 % after the others; with an SM in eight idle they
-  // end together, and the memory is as busy. 128 against 148 CTAs, us: one sequence
-  // of 131071 keys 85.7 / 91.9, 64 ragged ones of up to 16384 145.0 / 152.9, 64 of 2048
-  // 86.6 / 95.9, 32 of 4096 (head_dim 64) 48.6 / 52.5, 160 under a window of 1024 67.4 / 66.8.
-  const int sms = lw_host::sm_count();
-  d.grid = sms >= 32 ? sms / 32 * 32 : sms;
+  // Runs: a CTA per SM. Some groups of neighbouring SMs end 10 to 20 % after the
+  // others, which ones differs from GPU to GPU: 128 CTAs instead of 148 took 145 us
+  // instead of 153 for 64 ragged sequences on one B200 and 159 instead of 150 on another.
+  d.grid = lw_host::sm_count();
   // Clusters: the largest of 8, 4, 2 or 1 CTAs of which one per item runs at once,
   // when no sequence can give a CTA more than 1024 keys, or 512 where the items
   // fill less than 64 SMs (the runs then use more of them). Cluster / runs, us: 8 items of 2048 keys
