@@ -15,6 +15,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <string>
@@ -44,9 +45,14 @@ at::Tensor tensor(PyObject* o, const char* name, bool optional = false) {
 }
 
 long long whole(PyObject* o, const char* name) {
-  if (!PyLong_Check(o)) throw Refused{PyExc_TypeError, std::string(name) + " must be a whole number"};
+  PyObject* i = PyNumber_Index(o);
+  if (!i) {
+    PyErr_Clear();
+    throw Refused{PyExc_TypeError, std::string(name) + " must be a whole number"};
+  }
   int over = 0;
-  const long long v = PyLong_AsLongLongAndOverflow(o, &over);
+  const long long v = PyLong_AsLongLongAndOverflow(i, &over);
+  Py_DECREF(i);
   return over > 0 ? LLONG_MAX : over < 0 ? LLONG_MIN : v;
 }
 

@@ -543,6 +543,58 @@ def test_graphs():
     kernels.check_device_error()
 
 
+def test_two_threads():
+    """Calls of several host threads at once, each on its own stream."""
+    import threading
+    c = Batch([900, 40], 2, 128, 16, torch.float16)
+    q = torch.randn(2, 8, 128, generator=gen(2), device=DEV).half()
+    off = torch.tensor([0, 1, 2], dtype=torch.int32, device=DEV)
+    want = kernels.paged_attention(q, *c.cache()), kernels.prompt_attention(q, *c.cache(), off)
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work():
+        with torch.cuda.stream(torch.cuda.Stream(DEV)):
+            for _ in range(50):
+                got = kernels.paged_attention(q, *c.cache()), kernels.prompt_attention(q, *c.cache(), off)
+            torch.cuda.current_stream().synchronize()
+            if not all(torch.equal(a, b) for a, b in zip(got, want)):
+                wrong.append(1)
+
+    threads = [threading.Thread(target=work) for _ in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+def test_first_calls_of_a_process_may_be_captured():
+    import subprocess
+    import sys
+    code = """
+import torch
+from liteweight_b200 import kernels
+k = torch.randn(8, 2, 16, 64, device="cuda").half()
+table = torch.arange(8, device="cuda", dtype=torch.int32).view(2, 4)
+lens = torch.tensor([40, 64], device="cuda", dtype=torch.int32)
+off = torch.tensor([0, 1, 2], device="cuda", dtype=torch.int32)
+q = torch.randn(2, 4, 64, device="cuda").half()
+cos, sin = torch.ones(64, 64, device="cuda"), torch.zeros(64, 64, device="cuda")
+new = torch.zeros(2, 2, 64, device="cuda").half()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    r = kernels.qk_norm_rope(q, new, new, cos, sin, k, k.clone(), table, lens)
+    a, b = kernels.paged_attention(r, k, k, table, lens), kernels.prompt_attention(r, k, k, table, lens, off)
+g.replay()
+torch.cuda.synchronize()
+assert torch.equal(r, q) and (a.float() - b.float()).abs().max() < 4e-3
+kernels.check_device_error()
+"""
+    from pathlib import Path
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=120, cwd=Path(__file__).resolve().parent.parent)
+
+
 def test_empty_batches():
     c = Batch([5], 2, 64, 16, torch.float16)
     none = torch.empty(0, 4, 64, dtype=torch.float16, device=DEV)

@@ -125,6 +125,12 @@ def test_attention_asserts(kw):
         kernels.paged_attention(**tensors(**kw))
 
 
+@pytest.mark.parametrize("kw", [dict(window=2.5), dict(sinks="4"), dict(scale="x"), dict(q=None), dict(kv_lens=[1, 2])])
+def test_attention_types(kw):
+    with pytest.raises(TypeError):
+        kernels.paged_attention(**tensors(**kw))
+
+
 def test_prompt_attention_asserts():
     for off in (None, torch.zeros(3, dtype=torch.int64), torch.zeros(4, dtype=torch.int32),
                 torch.zeros(6, dtype=torch.int32)[::2]):
