@@ -72,7 +72,8 @@ void same_device(std::initializer_list<const at::Tensor*> ts) {
     if (!t->defined()) continue;
     if (!t->is_cuda())
       throw Refused{PyExc_RuntimeError,
-                    "liteweight_b200 ops run on CUDA tensors only (no CPU fallback); got a tensor on " + t->device().str()};
+                    "liteweight_b200 ops run on CUDA tensors only (no CPU fallback); got a tensor on " +
+                        t->device().str()};
   }
   for (const at::Tensor* t : ts) require(!t->defined() || t->device() == dev, "all tensors must be on one device");
 }

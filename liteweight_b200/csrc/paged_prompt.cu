@@ -41,6 +41,14 @@
 // rows that see it.
 //
 // Every wait is bounded; on expiry LW_ERR_TIMEOUT is recorded and the CTA ends.
+//
+// Measured (32 / 8 heads of 128): one prompt of 8192 tokens 540 us, 1.0 PFLOP/s, 0.6 of
+// the measured burst of a bf16 GEMM at an SM clock of 1.6 to 1.75 GHz under the
+// power limit; six prompts of 129 to 2111 tokens 252 us, 0.91 PFLOP/s. Per key tile
+// the tensor cores and the special-function unit (exponentials) need 2048 cycles
+// each for the two row tiles; a tile takes 3480: a row tile's softmax (2300) and
+// its way through the tensor cores (1160) follow one another, and two row tiles
+// overlap only so far.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -176,8 +184,8 @@ __device__ __noinline__ void add_nonfinite(const PromptParams& p, const PromptWo
         if (!(key <= pos && (key > lo || key < sinks))) continue;
         const int page = page_id(p.c, w.b, key);
         if (page < 0) continue;
-        const T* v = static_cast<const T*>(p.c.v) + page * p.c.vp + w.kvh * p.c.vh + (key & (p.c.page_size - 1)) * p.c.vs +
-                     8 * x;
+        const T* v = static_cast<const T*>(p.c.v) + page * p.c.vp + w.kvh * p.c.vh +
+                     (key & (p.c.page_size - 1)) * p.c.vs + 8 * x;
         for (int e = 0; e < 8; ++e) {
           const float f = static_cast<float>(v[e]);
           if (!isfinite(f)) o[e] = __float_as_uint(__uint_as_float(o[e]) + f);
@@ -194,7 +202,7 @@ template <int HD>
 struct PromptSmem {
   static constexpr int kTile = kPmKeys * HD * 2;              // a K, V or Q tile
   static constexpr int kSlots = HD == 128 ? 4 : 8;            // K and V tiles in the ring
-  static constexpr int kStage = 32 * 128;                     // a softmax warp's 32 rows, 128 bytes at a time, on their way out
+  static constexpr int kStage = 32 * 128;                     // a softmax warp's rows on their way out, 128 bytes at a time
   static constexpr int kBytes = 1024 + (2 + kSlots) * kTile + 8 * kStage;
 };
 
@@ -204,8 +212,8 @@ __global__ void __launch_bounds__(kPmThreads, 1) paged_prompt_kernel(const __gri
   constexpr int NS = S::kSlots, HALVES = HD / 64, HALF = kPmKeys * 128;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ __align__(16) uint4 clc_s;
-  __shared__ __align__(8) unsigned long long bar_q, bar_qfree, bar_full[NS], bar_empty[NS], bar_s[2], bar_p[2][2], bar_o[2],
-      bar_work, bar_taken, bar_clc, bar_done;
+  __shared__ __align__(8) unsigned long long bar_q, bar_qfree, bar_full[NS], bar_empty[NS], bar_s[2], bar_p[2][2],
+      bar_o[2], bar_work, bar_taken, bar_clc, bar_done;
   __shared__ PromptWork work_s;
   __shared__ uint32_t tmem_s;
   __shared__ volatile int abort_s, odd_s[4];   // odd_s[piece mod 4]: a value was cleared that rows see
@@ -313,8 +321,8 @@ __global__ void __launch_bounds__(kPmThreads, 1) paged_prompt_kernel(const __gri
             if (lane == 0) mbar_arrive_expect_tx(bar, S::kTile);
             __syncwarp();
             if (mine)
-              tma_load_4d(base + slot_at(s) + my_half * HALF + my_pg * pg * 128, kv ? &p.tm_v : &p.tm_k, my_half * 64, slot,
-                          w.kvh, from, bar);
+              tma_load_4d(base + slot_at(s) + my_half * HALF + my_pg * pg * 128, kv ? &p.tm_v : &p.tm_k, my_half * 64,
+                          slot, w.kvh, from, bar);
             __syncwarp();
             ++x;
             if (++s == NS) s = 0, phase ^= 1u;
@@ -361,8 +369,8 @@ __global__ void __launch_bounds__(kPmThreads, 1) paged_prompt_kernel(const __gri
         const uint64_t v = sw128_mn_desc(base + slot_at(s), HALF);
 #pragma unroll
         for (int x = x0; x < x1; ++x)
-          tc_mma_f16_ts(tmem + 2 * kPmKeys + g * HD, tmem + g * kPmKeys + 8 * x, v + (uint64_t)(x * (2048 >> 4)), kDescO,
-                        !first || x != 0);
+          tc_mma_f16_ts(tmem + 2 * kPmKeys + g * HD, tmem + g * kPmKeys + 8 * x, v + (uint64_t)(x * (2048 >> 4)),
+                        kDescO, !first || x != 0);
       };
       int s = 0, nq = 0, np[2] = {0, 0};   // ring slot, Q loads awaited, P tiles of each row tile awaited
       uint32_t phase = 0;
@@ -568,7 +576,7 @@ __global__ void __launch_bounds__(kPmThreads, 1) paged_prompt_kernel(const __gri
           uint32_t any = 0u;   // NaN in either half once an infinity or a NaN has passed: 0 * it
 #pragma unroll
           for (int c = 0; c < HALVES * 8; ++c) {
-            const uint4 v = lds128(row + (c / 8) * HALF + (((c + r) & 7) << 4));   // in any order: spread over the banks
+            const uint4 v = lds128(row + (c / 8) * HALF + (((c + r) & 7) << 4));   // an order that spreads over the banks
             any = Elem<T>::fma0(v.x, Elem<T>::fma0(v.y, Elem<T>::fma0(v.z, Elem<T>::fma0(v.w, any))));
           }
           if (has_nonfinite<T>(any)) {
@@ -784,7 +792,8 @@ cudaError_t prompt_launch(const lw::PromptParams& p, cudaStream_t s, bool pdl) {
 }
 
 // Tensor map of a pool [pages][heads][slots][head_dim] by its strides.
-bool pool_map(CUtensorMap* m, CUtensorMapDataType type, const void* base, const lw_paged_cache& c, const long long* st) {
+bool pool_map(CUtensorMap* m, CUtensorMapDataType type, const void* base, const lw_paged_cache& c,
+              const long long* st) {
   const uint64_t dims[4] = {(uint64_t)c.head_dim, (uint64_t)c.page_size, (uint64_t)c.n_kv_heads,
                             (uint64_t)std::max(1, c.n_pages)};
   const uint64_t strides[3] = {(uint64_t)st[2] * 2, (uint64_t)st[1] * 2, (uint64_t)st[0] * 2};

@@ -100,8 +100,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.T
     q_offsets[-1] on) are zero, or left as they were in a given `out`. New tokens
     must not share a slot.
     """
-    got = nat.bind().qk_norm_rope(q, k, v, cos, sin, k_pages, v_pages, page_table, kv_lens, q_offsets, q_weight, k_weight,
-                                  eps, out)
+    got = nat.bind().qk_norm_rope(q, k, v, cos, sin, k_pages, v_pages, page_table, kv_lens, q_offsets, q_weight,
+                                  k_weight, eps, out)
     if type(got) is int:
         nat.check("lw_qk_norm_rope", got)
     return got
