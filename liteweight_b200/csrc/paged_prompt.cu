@@ -31,7 +31,8 @@
 //
 // When the row tiles alone leave SMs idle (few rows, a long cache) the keys are
 // cut into slices as well; each writes (m, sum, fp32 O) to the workspace and a
-// second kernel joins them in order.
+// second kernel joins them in order. The launch knows only how long a context the
+// table can hold; a row tile that sees fewer keys takes fewer slices, or none.
 //
 // What hidden slots hold never reaches a result. Pages that no row sees are
 // zero-filled by the copy (their table entries are not read). In a tile that
@@ -65,6 +66,7 @@ constexpr int kPmThreads = 384;              // three warpgroups: softmax, softm
 constexpr int kPmSoftmaxRegs = 224, kPmOtherRegs = 56;
 static_assert(2 * 128 * kPmSoftmaxRegs + 128 * kPmOtherRegs <= 168 * kPmThreads, "registers of the launch");
 constexpr int kPmTmaWarp = 8, kPmMmaWarp = 9, kPmWorkWarp = 10;
+constexpr int kPmSliceTiles = 4;             // key tiles of a slice at least
 constexpr long long kPmWaitNs = 2000000000;
 constexpr float kPmGrow = 8.0f;              // log2 of the largest P
 constexpr int kPmPart = 96;                  // keys of P's first part
@@ -83,6 +85,7 @@ struct PromptParams {
   float scale_log2;
   int zero_tail;
   int slices;
+  int* part_n;            // [T][nq]: slices of the row (1: its result is written)
   float2* part_ml;        // [slices][T][nq]
   float* part_o;          // [slices][T][nq][head_dim]
 };
@@ -91,7 +94,7 @@ struct PromptParams {
 // against a slice of the key tiles they see.
 struct PromptWork {
   int valid;           // 0: there is no more
-  int kvh, slice, b;
+  int kvh, slice, slices, b;
   int tok0, np;        // first row of q, positions
   int pos0, last;      // position of the first, of the last
   int lo0;             // first key that the window of any row reaches
@@ -142,8 +145,10 @@ LW_DEV bool find_work(const PromptParams& p, int slot, int kvh, int slice, Promp
   w.w0 = w.lo0 / kPmKeys;
   w.ns = p.window > 0 ? min((min(p.sinks, w.lo0) + kPmKeys - 1) / kPmKeys, w.w0) : 0;
   const int all = w.last < 0 ? 0 : w.ns + w.last / kPmKeys + 1 - w.w0;
-  w.t0 = (int)((long long)all * slice / p.slices);
-  w.nt = (int)((long long)all * (slice + 1) / p.slices) - w.t0;
+  w.slices = max(1, min(p.slices, all / kPmSliceTiles));
+  if (slice >= w.slices) return false;
+  w.t0 = (int)((long long)all * slice / w.slices);
+  w.nt = (int)((long long)all * (slice + 1) / w.slices) - w.t0;
   return true;
 }
 
@@ -646,7 +651,8 @@ __global__ void __launch_bounds__(kPmThreads, 1) paged_prompt_kernel(const __gri
         __syncwarp();
       };
       auto put = [&](int c, uint4 v) { sts128(stage + lane * 128 + ((c ^ (lane & 7)) << 4), v); };
-      if (p.slices == 1) {
+      if (p.slices > 1 && w.slice == 0 && have) p.part_n[(long long)tok * p.nq + head] = w.slices;
+      if (w.slices == 1) {
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const long long row_at = have ? (tok * p.o_t + head * p.o_h) * 2 : -1ll;
 #pragma unroll 1
@@ -675,8 +681,7 @@ __global__ void __launch_bounds__(kPmThreads, 1) paged_prompt_kernel(const __gri
         }
       } else {
         const long long part = ((long long)w.slice * p.T + tok) * p.nq + head;
-        if (have) p.part_ml[part] = make_float2(w.nt > 0 ? m : -INFINITY, l);
-        if (w.nt == 0) continue;   // nothing else of this slice is read
+        if (have) p.part_ml[part] = make_float2(m, l);
 #pragma unroll 1
         for (int c0 = 0; c0 < HD; c0 += 32) {
           uint32_t o[32];
@@ -707,22 +712,41 @@ __global__ void __launch_bounds__(256) paged_prompt_join_kernel(const __grid_con
   const long long row = (long long)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
   if (row >= (long long)p.T * p.nq) return;
   const int tok = (int)(row / p.nq), head = (int)(row - (long long)tok * p.nq), d = (threadIdx.x % TPR) * 4;
-  if (row_sequence(p.off, p.c.B, tok) < 0) return;   // behind the last sequence: not ours
+  // four slices at a time; the first four are asked for before it is known how
+  // many there are (what is read for nothing is thrown away)
   const long long step = (long long)p.T * p.nq;
-  float M = -INFINITY;
-  for (int i = 0; i < p.slices; ++i) M = fmaxf(M, p.part_ml[i * step + row].x);
-  float L = 0.f;
+  const int said = p.part_n[row];
+  float2 ml[4];
+  float4 o[4];
+  auto load = [&](int i0, int n) {
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      ml[x] = make_float2(-INFINITY, 0.f);
+      if (i0 + x < n) {
+        ml[x] = p.part_ml[(i0 + x) * step + row];
+        o[x] = *reinterpret_cast<const float4*>(p.part_o + ((i0 + x) * step + row) * HD + d);
+      }
+    }
+  };
+  load(0, p.slices);
+  const int n = min(said, p.slices);
+  // its one slice wrote the result; behind the last sequence: not ours
+  if (n <= 1 || row_sequence(p.off, p.c.B, tok) < 0) return;
+  float M = -INFINITY, L = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i = 0; i < p.slices; ++i) {
-    const float2 ml = p.part_ml[i * step + row];
-    if (ml.x == -INFINITY) continue;   // a slice without a key for this row
-    const float f = ex2(ml.x - M);
-    const float4 o = *reinterpret_cast<const float4*>(p.part_o + (i * step + row) * HD + d);
-    L = fmaf(ml.y, f, L);
-    acc.x = fmaf(o.x, f, acc.x);
-    acc.y = fmaf(o.y, f, acc.y);
-    acc.z = fmaf(o.z, f, acc.z);
-    acc.w = fmaf(o.w, f, acc.w);
+  for (int i0 = 0; i0 < n; i0 += 4) {
+    if (i0) load(i0, n);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      if (i0 + x >= n || (ml[x].x == -INFINITY && ml[x].y == 0.f)) continue;   // a slice without a key for this row
+      const float mn = fmaxf(M, ml[x].x), f0 = ex2(M - mn), f1 = ex2(ml[x].x - mn);
+      M = mn;
+      L = fmaf(L, f0, ml[x].y * f1);
+      acc.x = fmaf(acc.x, f0, o[x].x * f1);
+      acc.y = fmaf(acc.y, f0, o[x].y * f1);
+      acc.z = fmaf(acc.z, f0, o[x].z * f1);
+      acc.w = fmaf(acc.w, f0, o[x].w * f1);
+    }
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;
   uint2 u = make_uint2(Elem<T>::pack(acc.x * inv, acc.y * inv), Elem<T>::pack(acc.z * inv, acc.w * inv));
@@ -755,7 +779,7 @@ int check(const lw_paged_attention_args* a) {
 
 struct PromptPlan {
   int group, rp, slices;
-  size_t o_off, bytes;
+  size_t ml_off, o_off, bytes;
 };
 
 PromptPlan prompt_plan(const lw_paged_attention_args* a) {
@@ -768,10 +792,11 @@ PromptPlan prompt_plan(const lw_paged_attention_args* a) {
   const long long ctas = ((long long)a->tokens + a->cache.batch * (R - 1)) / R * a->cache.n_kv_heads;
   long long keys = (long long)a->cache.table_width * a->cache.page_size;
   if (a->window > 0) keys = std::min(keys, (long long)a->window + a->sinks + R);
-  const long long most = std::min(keys / (4 * lw::kPmKeys), lw_host::sm_count() / std::max(1ll, ctas));
+  const long long most = std::min(keys / (lw::kPmSliceTiles * lw::kPmKeys), lw_host::sm_count() / std::max(1ll, ctas));
   d.slices = (int)std::max(1ll, std::min(most, 64ll));
   const size_t rows = (size_t)a->tokens * a->n_q_heads * d.slices;
-  d.o_off = (rows * sizeof(float2) + 255) & ~(size_t)255;
+  d.ml_off = ((size_t)a->tokens * a->n_q_heads * sizeof(int) + 255) & ~(size_t)255;
+  d.o_off = d.ml_off + ((rows * sizeof(float2) + 255) & ~(size_t)255);
   d.bytes = d.slices > 1 ? d.o_off + rows * a->cache.head_dim * sizeof(float) : 0;
   return d;
 }
@@ -838,7 +863,8 @@ int lw_paged_attention(const lw_paged_attention_args* a, lw_stream_t stream) {
   p.scale_log2 = a->scale * 1.4426950408889634f;
   p.zero_tail = a->zero_tail;
   p.slices = d.slices;
-  p.part_ml = static_cast<float2*>(a->workspace);
+  p.part_n = static_cast<int*>(a->workspace);
+  p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(a->workspace) + d.ml_off);
   p.part_o = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + d.o_off);
   const CUtensorMapDataType type =
       a->cache.dtype == LW_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;

@@ -303,6 +303,29 @@ def test_prompt(dtype, hd, nkv, group, name, page, window, sinks):
     assert torch.equal(out[:off[-1]], got[:off[-1]]) and (out[off[-1]:] == 3).all()   # left as they were
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (2000, 150)])
+def test_few_rows_of_short_and_long_contexts(hd, window, sinks):
+    """A table that can hold far more than the sequences do: the launch provides for
+    slices of the keys that only the long ones take; and the same for single tokens."""
+    lens, new = [300, 0, 40, 6000, 1], [20, 0, 5, 33, 1]
+    c = Batch(lens, 1, hd, 16, torch.bfloat16)
+    wide = torch.full((5, 5000), -7, dtype=torch.int32, device=DEV)
+    wide[:, :c.table.shape[1]] = c.table
+    off = [0, 20, 20, 25, 58, 59]
+    q = torch.randn(62, 4, hd, generator=gen(4), device=DEV).bfloat16()
+    offs = torch.tensor(off, dtype=torch.int32, device=DEV)
+    got = kernels.prompt_attention(q, c.k_pages, c.v_pages, wide, c.kv_lens, offs, window=window, sinks=sinks)
+    one = kernels.paged_attention(q[:5], c.k_pages, c.v_pages, wide, c.kv_lens, window=window, sinks=sinks)
+    kernels.check_device_error()
+    assert (got[59:] == 0).all() and (one[1] == 0).all()
+    for b, n in enumerate(lens):
+        if n:
+            rows = slice(off[b], off[b + 1])
+            check(got[rows], *attend(q[rows], c.k[b], c.v[b], n - new[b], window, sinks, hd ** -0.5, torch.bfloat16))
+            check(one[b:b + 1], *attend(q[b:b + 1], c.k[b], c.v[b], n - 1, window, sinks, hd ** -0.5, torch.bfloat16))
+
+
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("window,sinks", [(None, 0), (40, 3)])
