@@ -523,7 +523,19 @@ __global__ void __launch_bounds__(kPdThreads) paged_join_kernel(const PagedDecod
   const int H = p.c.nkv * p.hblocks, r = blockIdx.y;
   pdl_wait();
   pdl_launch_dependents();
+  // piece i of the item that may begin here; a warp's first is asked for before it
+  // is known whether there is one (what is read for nothing is thrown away)
+  float2 ml[4];
+  float v[4][V];
+  auto load = [&](int x, int i) {
+    const float* s = p.part + (long long)(i == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + i)) * S::kPiece +
+                     r * S::kStride;
+    ml[x] = *reinterpret_cast<const float2*>(s + HD);
+    if constexpr (V == 4) *reinterpret_cast<float4*>(v[x]) = *reinterpret_cast<const float4*>(s + d);
+    else *reinterpret_cast<float2*>(v[x]) = *reinterpret_cast<const float2*>(s + d);
+  };
   const int2 mt = p.meta[blockIdx.x];
+  if (blockIdx.x + warp < gridDim.x) load(0, warp);
   for (int b = blockIdx.x + (int)gridDim.x * warp; b < p.c.B; b += (int)gridDim.x * kPdWarps)
     if (seq_len(p.c, b) == 0)
       for (int h = r; h < p.c.nkv * p.group; h += gridDim.y) {
@@ -533,26 +545,15 @@ __global__ void __launch_bounds__(kPdThreads) paged_join_kernel(const PagedDecod
       }
   const int b = mt.x / H, hh = mt.x - b * H, kvh = hh / p.hblocks, hb = hh - kvh * p.hblocks;
   if (mt.y == 0 || r >= p.group - hb * ROWS) return;
-  constexpr int kAtOnce = 4;
   float M = -INFINITY, L = 0.f, acc[V] = {};
-  for (int i0 = warp; i0 < mt.y; i0 += kPdWarps * kAtOnce) {
-    float2 ml[kAtOnce];
-    float v[kAtOnce][V];
+  for (int i0 = warp; i0 < mt.y; i0 += kPdWarps * 4) {
 #pragma unroll
-    for (int x = 0; x < kAtOnce; ++x) {
-      const int i = i0 + x * kPdWarps;
-      ml[x] = make_float2(-INFINITY, 0.f);
-      if (i < mt.y) {
-        const float* s = p.part + (long long)(i == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + i)) * S::kPiece +
-                         r * S::kStride;
-        ml[x] = *reinterpret_cast<const float2*>(s + HD);
-        if constexpr (V == 4) *reinterpret_cast<float4*>(v[x]) = *reinterpret_cast<const float4*>(s + d);
-        else *reinterpret_cast<float2*>(v[x]) = *reinterpret_cast<const float2*>(s + d);
-      }
-    }
+    for (int x = 0; x < 4; ++x)
+      if ((x > 0 || i0 != warp) && i0 + x * kPdWarps < mt.y) load(x, i0 + x * kPdWarps);
 #pragma unroll
-    for (int x = 0; x < kAtOnce; ++x) {
-      if (ml[x].x == -INFINITY && ml[x].y == 0.f) continue;   // past the end, or no key seen in the piece
+    for (int x = 0; x < 4; ++x) {
+      // past the last, or no key seen in the piece
+      if (i0 + x * kPdWarps >= mt.y || (ml[x].x == -INFINITY && ml[x].y == 0.f)) continue;
       const float mn = fmaxf(M, ml[x].x);
       const float f0 = ex2(M - mn), f1 = ex2(ml[x].x - mn);
       M = mn;
