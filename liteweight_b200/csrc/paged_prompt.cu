@@ -48,8 +48,9 @@
 // power limit; six prompts of 129 to 2111 tokens 252 us, 0.91 PFLOP/s. Per key tile
 // the tensor cores and the special-function unit (exponentials) need 2048 cycles
 // each for the two row tiles; a tile takes 3480: a row tile's softmax (2300) and
-// its way through the tensor cores (1160) follow one another, and two row tiles
-// overlap only so far.
+// its way through the tensor cores (1160) follow one another. Making S before it
+// is waited for did not shorten it (526 -> 575 us): the bound is what two softmax
+// warps per scheduler get through. Four (two threads per row) were slower (685).
 #include <algorithm>
 
 #include "paged.cuh"

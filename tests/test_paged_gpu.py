@@ -628,4 +628,6 @@ def test_empty_batches():
     assert (kernels.prompt_attention(rows, *c.cache(), off) == 0).all()
     assert (kernels.paged_attention(rows, c.k_pages[:0], c.v_pages[:0], torch.empty(3, 0, dtype=torch.int32, device=DEV),
                                     torch.zeros(3, dtype=torch.int32, device=DEV)) == 0).all()
+    assert (kernels.prompt_attention(rows, c.k_pages[:0], c.v_pages[:0], torch.empty(1, 0, dtype=torch.int32, device=DEV),
+                                     torch.zeros(1, dtype=torch.int32, device=DEV), off) == 0).all()
     kernels.check_device_error()
