@@ -20,6 +20,11 @@ struct Elem<__half> {
   static LW_DEV uint32_t pack(float lo, float hi) { return h2_as_u32(__floats2half2_rn(lo, hi)); }
   static LW_DEV float2 unpack(uint32_t u) { return __half22float2(u32_as_h2(u)); }
   static constexpr uint32_t kExpMask = 0x7C00u;   // all ones: infinity or NaN
+  // Softmax weights rounded to fp16 may be up to 2^15 (the largest fp16 is just
+  // below 2^16): below 2^-14 the type has a fixed step, and with the weights in
+  // [0, 1] those under 2^-25 would be 0 in the product and still count in the sum
+  // (131070 of e^-18 beside a 1: the result would be 0 instead of 0.002).
+  static constexpr float kMaxWeightLog2 = 15.0f;
   // a * 0 + c in each half
   static LW_DEV uint32_t fma0(uint32_t a, uint32_t c) {
     uint32_t d;
@@ -38,6 +43,7 @@ struct Elem<__nv_bfloat16> {
     return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
   }
   static constexpr uint32_t kExpMask = 0x7F80u;
+  static constexpr float kMaxWeightLog2 = 0.0f;   // the range of fp32: small weights keep their precision
   static LW_DEV uint32_t fma0(uint32_t a, uint32_t c) {
     uint32_t d;
     asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(0u), "r"(c));

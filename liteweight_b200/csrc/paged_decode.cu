@@ -92,7 +92,8 @@ struct DecodeShape {
 };
 
 // One warp's share of an item: queries as MMA fragments, the online softmax of
-// rows g and g + 8 (g + 8 with ROWS = 16 only), the accumulator.
+// rows g and g + 8 (g + 8 with ROWS = 16 only), the accumulator. m is the base of
+// the weights: the maximum so far less kMaxWeightLog2.
 template <typename T, int HD, int ROWS>
 struct WarpItem {
   using S = DecodeShape<HD, ROWS>;
@@ -164,7 +165,10 @@ struct WarpItem {
       for (int n = 1; n < N; ++n) mx = fmaxf(mx, fmaxf(sc[n][2 * r], sc[n][2 * r + 1]));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float mn = fmaxf(m[r], mx * p.scale_log2);
+      // the base that weights are taken from: the maximum less the largest weight's
+      // exponent, rounded up, so that no weight is above 2^kMaxWeightLog2 however
+      // coarse fp32 is at the scores' size. Sums and accumulators carry the factor.
+      const float mn = fmaxf(m[r], __fmaf_ru(mx, p.scale_log2, -Elem<T>::kMaxWeightLog2));
       const float base = mn == -INFINITY ? 0.f : mn;   // no key seen yet: every weight is 0
       corr[r] = ex2(m[r] - base);
       m[r] = mn;
@@ -191,8 +195,9 @@ struct WarpItem {
     const int r0 = ((lane >> 3) & 1) * 8 + (lane & 7), cb = lane >> 4;
 #pragma unroll
     for (int x = 0; x < S::kGroups; ++x) {
-      // the weights lie in [0, 1]: rounded to T for the second product, half a
-      // step each, averaged over the keys; their sum stays in fp32
+      // rounded to T for the second product, half a step each, averaged over the
+      // keys (fp16: weights under 2^-29 of the largest so far by up to 2^-40 of it);
+      // their sum stays in fp32
       const uint32_t a0 = Elem<T>::pack(sc[2 * x][0], sc[2 * x][1]);
       const uint32_t a2 = Elem<T>::pack(sc[2 * x + 1][0], sc[2 * x + 1][1]);
       const uint32_t a1 = R == 2 ? Elem<T>::pack(sc[2 * x][2], sc[2 * x][3]) : 0u;

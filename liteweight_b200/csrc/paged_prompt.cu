@@ -14,8 +14,8 @@
 //   warps 0-3, 4-7  softmax of row tile 0 / 1, one row per thread: read S, mask,
 //                   keep the running maximum and sum in fp32, write P. The
 //                   accumulator is rescaled only when a row's maximum has grown
-//                   by more than 2^8 (P stays below 256, exact in range; the
-//                   sum and O carry the same factor), so O rarely moves.
+//                   by more than 2^8 (P stays within the type's range; the sum
+//                   and O carry the same factor), so O rarely moves.
 //   warp 8          TMA copies: Q once, K and V tiles page by page into a ring.
 //   warp 9          issues tcgen05.mma: S_g = Q_g K^T (both from shared memory),
 //                   O_g += P_g V (P from tensor memory). While one row tile is in
@@ -69,7 +69,11 @@ static_assert(2 * 128 * kPmSoftmaxRegs + 128 * kPmOtherRegs <= 168 * kPmThreads,
 constexpr int kPmTmaWarp = 8, kPmMmaWarp = 9, kPmWorkWarp = 10;
 constexpr int kPmSliceTiles = 4;             // key tiles of a slice at least
 constexpr long long kPmWaitNs = 2000000000;
-constexpr float kPmGrow = 8.0f;              // log2 of the largest P
+constexpr float kPmGrow = 8.0f;              // log2 of what a row's maximum may grow by before O is rescaled
+// log2 of the largest P against the maximum it was taken from: fp16 leaves the
+// range above 1 that growth does not need to small weights
+template <typename T>
+constexpr float kPmMaxWeightLog2 = Elem<T>::kMaxWeightLog2 > kPmGrow ? Elem<T>::kMaxWeightLog2 - kPmGrow : 0.0f;
 constexpr int kPmPart = 96;                  // keys of P's first part
 
 struct PromptParams {
@@ -552,11 +556,12 @@ __global__ void __launch_bounds__(kPmThreads, 1) paged_prompt_kernel(const __gri
           mx[x] = max3(mx[x], mx[x], __uint_as_float(s[x][31]));
         }
         // a NaN among the row's scores makes its maximum, and so all of the row, NaN
-        const float mt = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * p.scale_log2;
+        // (the base of the weights, rounded up: none is above 2^kPmMaxWeightLog2)
+        const float mt = __fmaf_ru(max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]), p.scale_log2, -kPmMaxWeightLog2<T>);
         if (i == 0) {
           m = have ? mt : 0.f;   // a row that is none holds anything
         } else {
-          const bool grow = have && !(mt <= m + kPmGrow);
+          const bool grow = have && !(mt <= __fadd_rd(m, kPmGrow));
           if (__any_sync(0xffffffffu, grow)) {
             // O's update i - 1 is complete (S(i) was issued after it)
             const float f = !grow ? 1.f : (m == -INFINITY ? 0.f : ex2(m - mt));
@@ -596,7 +601,8 @@ __global__ void __launch_bounds__(kPmThreads, 1) paged_prompt_kernel(const __gri
         const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), sub2 = make_float2(-sub, -sub);
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         // weights rounded to T for the second product: half a step each, averaged
-        // over the keys; their sum is that of the unrounded ones
+        // over the keys (fp16: weights under 2^-21 of the base's maximum by up to
+        // 2^-32 of it); their sum is that of the unrounded ones
         auto weights = [&](int e) {
           const int x = e / 16, y = (2 * e) % 32;
           float2 a = fma2(make_float2(__uint_as_float(s[x][y]), __uint_as_float(s[x][y + 1])), scale2, sub2);
