@@ -164,6 +164,16 @@ LW_DEV int page_id(const PagedView& c, int b, int tok) {
   return -1;
 }
 
+// The base of a row that sees keys, every score of which is minus infinity: below
+// any other, above that of a row (or a part of one) that sees none.
+constexpr float kAllBelow = -3.402823466e38f;
+
+// 1 / the sum of the weights; 0 for a row that sees no key, NaN (a softmax of
+// minus infinities) for one that sees only keys without weight.
+LW_DEV float weight_inverse(float m, float l) {
+  return l != 0.f ? 1.f / l : m == -INFINITY ? 0.f : __int_as_float(0x7FFFFFFF);
+}
+
 // The first key that position p sees through its window.
 LW_DEV int window_start(int p, int window) { return window > 0 ? max(0, p - window + 1) : 0; }
 

@@ -101,6 +101,7 @@ struct WarpItem {
   uint32_t qa[HD / 16][2 * R];
   float o[HD / 8][4];
   float m[R], l[R];
+  bool seen;   // a visible key was there
 
   LW_DEV static void load_q(const PagedDecodeParams& p, int b, int head0, int rows, int lane,
                             uint32_t (&f)[HD / 16][2 * R]) {
@@ -122,6 +123,7 @@ struct WarpItem {
     for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 #pragma unroll
     for (int r = 0; r < R; ++r) m[r] = -INFINITY, l[r] = 0.f;
+    seen = false;
   }
 
   // The keys from key0 on, in the stage at `kt` (K tile, then V tile; 16-byte chunk
@@ -129,6 +131,7 @@ struct WarpItem {
   LW_DEV void tile(const PagedDecodeParams& p, const TileSpan& sp, int key0, uint32_t lost, uint32_t kt, int lane) {
     constexpr int N = S::kTile / 8;   // score fragments of 8 keys
     const int t = lane & 3;
+    seen |= lost != (1u << S::kGroups) - 1u;
     float sc[N][4];
 #pragma unroll
     for (int n = 0; n < N; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
@@ -216,6 +219,7 @@ struct WarpItem {
   LW_DEV void finish_sums() {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
+      if (seen) m[r] = fmaxf(m[r], kAllBelow);
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
     }
@@ -242,7 +246,7 @@ struct WarpItem {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       if (g + 8 * r >= rows) continue;
-      const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
+      const float inv = weight_inverse(m[r], l[r]);
       T* dst = static_cast<T*>(p.out) + b * p.o_b + (long long)(head0 + g + 8 * r) * p.o_h + 2 * t;
 #pragma unroll
       for (int i = 0; i < HD / 8; ++i)
@@ -252,7 +256,8 @@ struct WarpItem {
 };
 
 // The warp's copy of a tile into a ring stage, zeros for keys nobody sees. Returns
-// the 16-key groups whose page id is outside the pool: their keys are hidden.
+// the 16-key groups without a visible key: those whose page id is outside the pool
+// and, of a tile of two, one that lies outside what is seen.
 template <typename T, int HD, int ROWS>
 LW_DEV uint32_t copy_tile(const PagedDecodeParams& p, const TileSpan& sp, int b, int key0, int kvh, uint32_t dst,
                           int lane) {
@@ -266,7 +271,7 @@ LW_DEV uint32_t copy_tile(const PagedDecodeParams& p, const TileSpan& sp, int b,
     const int first = key0 + 16 * x;   // a group may lie outside what is seen: its table entry is not read
     const bool seen = S::kGroups == 1 || (first < sp.len && (first + 16 > sp.lo || first < sp.sinks));
     page[x] = seen ? page_id(p.c, b, first) : 0;
-    if (page[x] < 0) lost |= 1u << x;
+    if (!seen || page[x] < 0) lost |= 1u << x;
   }
 #pragma unroll
   for (int x = 0; x < S::kGroups; ++x) {
@@ -377,7 +382,7 @@ __global__ void __launch_bounds__(kPdThreads, 1) paged_decode_kernel(const Paged
     };
     const uint32_t ring = smem_u32(smem) + warp * S::kRing;
     LineCursor ahead = cur;
-    uint32_t lost = 0;   // kGroups bits per stage: page ids outside the pool
+    uint32_t lost = 0;   // kGroups bits per stage: groups without a visible key
     auto issue = [&](long long tile, int st) {
       if (tile < r1) {
         if (tile >= ahead.item0 + ahead.span.nt) advance(ahead);
@@ -501,7 +506,7 @@ __global__ void __launch_bounds__(kPdThreads, 1) paged_decode_kernel(const Paged
     }
     const bool starts = e0 & 1;
     if (starts && !__shfl_sync(0xffffffffu, my_runs, e0)) {
-      const float inv = L == 0.f ? 0.f : 1.f / L;
+      const float inv = weight_inverse(M, L);
       T* out = static_cast<T*>(p.out) + b * p.o_b + (long long)(kvh * p.group + hb * ROWS + r) * p.o_h + lane * V;
 #pragma unroll
       for (int i = 0; i < V / 2; ++i)
@@ -588,7 +593,7 @@ __global__ void __launch_bounds__(kPdThreads) paged_join_kernel(const PagedDecod
 #pragma unroll
     for (int e = 0; e < V; ++e) acc[e] = fmaf(sm_acc[w][d + e], f, acc[e]);
   }
-  const float inv = L == 0.f ? 0.f : 1.f / L;
+  const float inv = weight_inverse(M, L);
   T* dst = static_cast<T*>(p.out) + b * p.o_b + (long long)(kvh * p.group + hb * ROWS + r) * p.o_h + d;
   if constexpr (V == 4)
     *reinterpret_cast<uint2*>(dst) = make_uint2(Elem<T>::pack(acc[0] * inv, acc[1] * inv),
@@ -689,7 +694,7 @@ __global__ void __launch_bounds__(kPdThreads, 1) paged_decode_cluster_kernel(con
       x0 = fmaf(v[c].x, f, x0);
       x1 = fmaf(v[c].y, f, x1);
     }
-    const float inv = L == 0.f ? 0.f : 1.f / L;
+    const float inv = weight_inverse(M, L);
     T* dst = static_cast<T*>(p.out) + b * p.o_b + (long long)(head0 + r) * p.o_h + d;
     *reinterpret_cast<uint32_t*>(dst) = Elem<T>::pack(x0 * inv, x1 * inv);
   }

@@ -208,6 +208,16 @@ __device__ __noinline__ void add_nonfinite(const PromptParams& p, const PromptWo
   tmem_wait_st();
 }
 
+// Whether the piece's tiles hold a key that the row sees (asked for a row without a weight).
+__device__ __noinline__ bool sees_key(const PromptParams& p, const PromptWork& w, int pos, int lo, int sinks) {
+  for (int i = 0; i < w.nt; ++i) {
+    const int key0 = w.key_of(i);
+    for (int key = key0; key < key0 + kPmKeys && key <= pos; key += 16)   // 16 keys are of one page
+      if ((min(key + 15, pos) > lo || key < sinks) && page_id(p.c, w.b, key) >= 0) return true;
+  }
+  return false;
+}
+
 template <int HD>
 struct PromptSmem {
   static constexpr int kTile = kPmKeys * HD * 2;              // a K, V or Q tile
@@ -642,6 +652,7 @@ __global__ void __launch_bounds__(kPmThreads, 1) paged_prompt_kernel(const __gri
         tc_fence_after();
       }
       if (odd_s[it & 3]) add_nonfinite<T, HD>(p, w, pos, lo, sinks, to);
+      if (have && m == -INFINITY && sees_key(p, w, pos, lo, sinks)) m = kAllBelow;
       const int tok = w.tok0 + g * p.rp + r_pos, head = w.kvh * p.group + r_head;
       // 128 bytes of each of the warp's 32 rows at a time go through shared memory
       // (16-byte chunk c of a row at chunk c ^ (row & 7)), so that eight lanes
@@ -660,7 +671,7 @@ __global__ void __launch_bounds__(kPmThreads, 1) paged_prompt_kernel(const __gri
       auto put = [&](int c, uint4 v) { sts128(stage + lane * 128 + ((c ^ (lane & 7)) << 4), v); };
       if (p.slices > 1 && w.slice == 0 && have) p.part_n[(long long)tok * p.nq + head] = w.slices;
       if (w.slices == 1) {
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const float inv = weight_inverse(m, l);
         const long long row_at = have ? (tok * p.o_t + head * p.o_h) * 2 : -1ll;
 #pragma unroll 1
         for (int c0 = 0; c0 < HD; c0 += 64) {
@@ -755,7 +766,7 @@ __global__ void __launch_bounds__(256) paged_prompt_join_kernel(const __grid_con
       acc.w = fmaf(acc.w, f0, o[x].w * f1);
     }
   }
-  const float inv = L == 0.f ? 0.f : 1.f / L;
+  const float inv = weight_inverse(M, L);
   uint2 u = make_uint2(Elem<T>::pack(acc.x * inv, acc.y * inv), Elem<T>::pack(acc.z * inv, acc.w * inv));
   *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + tok * p.o_t + head * p.o_h + d) = u;
 }

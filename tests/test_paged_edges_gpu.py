@@ -87,3 +87,121 @@ def test_huge_scores(dtype, hd, size):
         check(kernels.paged_attention(q[:1], *c.cache()), want[:1], tol[:1])
         check(kernels.prompt_attention(q, *c.cache(), offsets(2)), want, tol)
     kernels.check_device_error()
+
+
+# ------------------------------------------------------------------ infinities and NaN that are seen
+
+# a cluster per item; runs whose items lie within one; a long item cut by CTAs; both with a wide group
+DECODE_FORMS = {"cluster": ([300, 77], 4), "cluster-wide": ([900], 12), "runs": ([200 + i % 9 for i in range(700)], 4),
+                "join": ([20000, 77], 4), "join-wide": ([9000], 12)}
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("form", DECODE_FORMS)
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_decode_shows_the_infinities_and_nans_that_it_sees(dtype, hd, form, value):
+    """A value's infinity or NaN reaches its own dim of the rows that see it and
+    nothing else; a key's NaN the whole row of its kv head."""
+    lens, group = DECODE_FORMS[form]
+    c = Batch(lens, 2, hd, 16, dtype)
+    q = torch.randn(len(lens), 2 * group, hd, generator=gen(3), device=DEV).to(dtype)
+    dims = torch.arange(hd, device=DEV) != 5
+    n = lens[0]
+    want, tol = attend(q[:1], c.k[0], c.v[0], n - 1, None, 0, hd ** -0.5, dtype)
+    others = kernels.paged_attention(q, *c.cache())[1:]
+    for key in (0, 17, n // 2, n - 1):
+        k, v = c.k[0].clone(), c.v[0].clone()
+        v[key, 1, 5] = value
+        c.put(0, 0, k, v)
+        got = kernels.paged_attention(q, *c.cache())
+        x = got[0, group:, 5].float()
+        assert (x.isnan() if math.isnan(value) else x == value).all(), "a visible value was lost"
+        check(got[:1, :, dims], want[:, :, dims], tol[:, :, dims])
+        check(got[:1, :group], want[:, :group], tol[:, :group])
+        assert torch.equal(got[1:], others)
+        k[key, 1, 7] = float("nan")
+        c.put(0, 0, k, c.v[0])
+        got = kernels.paged_attention(q, *c.cache())
+        assert got[0, group:].isnan().all()
+        check(got[:1, :group], want[:, :group], tol[:, :group])
+        assert torch.equal(got[1:], others)
+    kernels.check_device_error()
+
+
+def all_below(c, b, keys):
+    """Keys whose score is minus infinity for queries with q[..., 0] > 0."""
+    k = c.k[b].clone()
+    k[keys, :, 0] = -float("inf")
+    c.put(b, 0, k, c.v[b])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("form", DECODE_FORMS)
+def test_scores_of_minus_infinity(dtype, hd, form):
+    """Such a key has no weight beside others; a row that sees only such keys is
+    NaN, as a softmax of them is, where one that sees no key is zero."""
+    lens, group = DECODE_FORMS[form]
+    c = Batch(lens, 1, hd, 16, dtype)
+    q = torch.randn(len(lens), group, hd, generator=gen(3), device=DEV).to(dtype)
+    q[..., 0] = q[..., 0].abs() + 0.1
+    n = lens[0]
+    others = kernels.paged_attention(q, *c.cache())[1:]
+    kept = torch.tensor([2, n // 2, n - 2], device=DEV)
+    gone = torch.ones(n, dtype=torch.bool, device=DEV)
+    gone[kept] = False
+    all_below(c, 0, gone)
+    want, tol = attend(q[:1], c.k[0][kept], c.v[0][kept], 2, None, 0, hd ** -0.5, dtype)
+    got = kernels.paged_attention(q, *c.cache())
+    check(got[:1], want, tol)
+    assert torch.equal(got[1:], others)
+    all_below(c, 0, slice(None))
+    got = kernels.paged_attention(q, *c.cache())
+    assert got[0].isnan().all() and torch.equal(got[1:], others)
+    kernels.check_device_error()
+    c.table[0] = -1   # nothing is visible then
+    got = kernels.paged_attention(q, *c.cache())
+    assert (got[0] == 0).all()
+    with pytest.raises(Exception, match="out of range"):
+        kernels.check_device_error()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (40, 3)])
+@pytest.mark.parametrize("width", [40, 2000])
+def test_scores_of_minus_infinity_in_prompts(dtype, hd, window, sinks, width):
+    """With the wide table the rows' keys are cut into slices."""
+    n, rows = 600, 90
+    c = Batch([n], 1, hd, 16, dtype)
+    wide = torch.full((1, width), -5, dtype=torch.int32, device=DEV)
+    wide[:, :-(-n // 16)] = c.table[:, :-(-n // 16)]
+    cache = (c.k_pages, c.v_pages, wide, c.kv_lens)
+    q = torch.randn(rows, 3, hd, generator=gen(3), device=DEV).to(dtype)
+    q[..., 0] = q[..., 0].abs() + 0.1
+    p = torch.arange(n - rows, n, device=DEV)
+    for kept in ([550], [1, 530, 599], []):
+        gone = torch.ones(n, dtype=torch.bool, device=DEV)
+        gone[kept] = False
+        all_below(c, 0, gone)
+        got = kernels.prompt_attention(q, *cache, offsets(rows), window=window, sinks=sinks)
+        j = torch.tensor(kept, device=DEV, dtype=torch.int64)[None]
+        seen = (j <= p[:, None]) & ((p[:, None] - j < window) | (j < sinks) if window else True)
+        some = seen.any(-1)
+        for i in range(rows):
+            if not some[i]:
+                assert got[i].isnan().all(), i
+        for mask in seen[some].unique(dim=0) if kept else ():
+            at = (seen == mask).all(-1)
+            use = torch.tensor(kept, device=DEV)[mask]
+            # every row of the group sees all of `use`
+            first = [attend(q[i:i + 1], c.k[0][use], c.v[0][use], len(use) - 1, None, 0, hd ** -0.5, dtype)
+                     for i in at.nonzero()[:, 0].tolist()]
+            check(got[at], torch.cat([x[0] for x in first]), torch.cat([x[1] for x in first]))
+    kernels.check_device_error()
+    c.table[0] = -1
+    got = kernels.prompt_attention(q, *c.cache(), offsets(rows), window=window, sinks=sinks)
+    assert (got == 0).all()
+    with pytest.raises(Exception, match="out of range"):
+        kernels.check_device_error()
