@@ -77,6 +77,20 @@ LW_DEV int tile_key(const TileSpan& s, int tile) {
   return (tile < s.ns ? tile : s.w0 + tile - s.ns) * TILE;
 }
 
+// Whether tiles t0, t0 + step, .. below t1 hold a visible key. Asked only for a row
+// that has no weight, so that the tiles' loop does not track it.
+template <int TILE>
+LW_DEV bool sees_key(const PagedDecodeParams& p, const TileSpan& sp, int b, int t0, int t1, int step) {
+#pragma unroll 1
+  for (int tile = t0; tile < t1; tile += step)
+#pragma unroll 1
+    for (int x = 0; x < TILE; x += 16) {   // 16 keys are of one page
+      const int key = tile_key<TILE>(sp, tile) + x;
+      if (key < sp.len && (key + 16 > sp.lo || key < sp.sinks) && page_id(p.c, b, key) >= 0) return true;
+    }
+  return false;
+}
+
 // Sizes of a kernel's shared memory: a ring per warp, then pieces [warps][ROWS][HD + 8]
 // (accumulator, maximum, sum; the stride keeps the fragment stores off each other's banks).
 template <int HD, int ROWS>
@@ -101,7 +115,6 @@ struct WarpItem {
   uint32_t qa[HD / 16][2 * R];
   float o[HD / 8][4];
   float m[R], l[R];
-  bool seen;   // a visible key was there
 
   LW_DEV static void load_q(const PagedDecodeParams& p, int b, int head0, int rows, int lane,
                             uint32_t (&f)[HD / 16][2 * R]) {
@@ -123,7 +136,6 @@ struct WarpItem {
     for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 #pragma unroll
     for (int r = 0; r < R; ++r) m[r] = -INFINITY, l[r] = 0.f;
-    seen = false;
   }
 
   // The keys from key0 on, in the stage at `kt` (K tile, then V tile; 16-byte chunk
@@ -131,7 +143,6 @@ struct WarpItem {
   LW_DEV void tile(const PagedDecodeParams& p, const TileSpan& sp, int key0, uint32_t lost, uint32_t kt, int lane) {
     constexpr int N = S::kTile / 8;   // score fragments of 8 keys
     const int t = lane & 3;
-    seen |= lost != (1u << S::kGroups) - 1u;
     float sc[N][4];
 #pragma unroll
     for (int n = 0; n < N; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
@@ -216,10 +227,11 @@ struct WarpItem {
     }
   }
 
-  LW_DEV void finish_sums() {
+  // Of tiles t0, t0 + step, .. below t1 of sequence b.
+  LW_DEV void finish(const PagedDecodeParams& p, const TileSpan& sp, int b, int t0, int t1, int step) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      if (seen) m[r] = fmaxf(m[r], kAllBelow);
+      if (m[r] == -INFINITY && sees_key<S::kTile>(p, sp, b, t0, t1, step)) m[r] = kAllBelow;
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
     }
@@ -256,8 +268,7 @@ struct WarpItem {
 };
 
 // The warp's copy of a tile into a ring stage, zeros for keys nobody sees. Returns
-// the 16-key groups without a visible key: those whose page id is outside the pool
-// and, of a tile of two, one that lies outside what is seen.
+// the 16-key groups whose page id is outside the pool: their keys are hidden.
 template <typename T, int HD, int ROWS>
 LW_DEV uint32_t copy_tile(const PagedDecodeParams& p, const TileSpan& sp, int b, int key0, int kvh, uint32_t dst,
                           int lane) {
@@ -271,7 +282,7 @@ LW_DEV uint32_t copy_tile(const PagedDecodeParams& p, const TileSpan& sp, int b,
     const int first = key0 + 16 * x;   // a group may lie outside what is seen: its table entry is not read
     const bool seen = S::kGroups == 1 || (first < sp.len && (first + 16 > sp.lo || first < sp.sinks));
     page[x] = seen ? page_id(p.c, b, first) : 0;
-    if (!seen || page[x] < 0) lost |= 1u << x;
+    if (page[x] < 0) lost |= 1u << x;
   }
 #pragma unroll
   for (int x = 0; x < S::kGroups; ++x) {
@@ -382,7 +393,7 @@ __global__ void __launch_bounds__(kPdThreads, 1) paged_decode_kernel(const Paged
     };
     const uint32_t ring = smem_u32(smem) + warp * S::kRing;
     LineCursor ahead = cur;
-    uint32_t lost = 0;   // kGroups bits per stage: groups without a visible key
+    uint32_t lost = 0;   // kGroups bits per stage: page ids outside the pool
     auto issue = [&](long long tile, int st) {
       if (tile < r1) {
         if (tile >= ahead.item0 + ahead.span.nt) advance(ahead);
@@ -417,6 +428,7 @@ __global__ void __launch_bounds__(kPdThreads, 1) paged_decode_kernel(const Paged
         Item::load_q(p, nxt.b, head_of(nxt), rows_of(nxt), lane, qn);
       }
       w.clear();
+      const int t0 = (int)(tile - cur.item0);
       for (; tile < end; ++tile) {
         cp_async_wait<S::kStages - 1>();   // the oldest group has landed
         __syncwarp();
@@ -426,7 +438,7 @@ __global__ void __launch_bounds__(kPdThreads, 1) paged_decode_kernel(const Paged
         issue(next++, st);
         if (++st == S::kStages) st = 0;
       }
-      w.finish_sums();
+      w.finish(p, cur.span, cur.b, t0, (int)(end - cur.item0), 1);
       const int item = cur.b * H + cur.hh;
       if (starts && ends) {
         w.store_out(p, cur.b, head_of(cur), rows_of(cur), lane);
@@ -648,7 +660,7 @@ __global__ void __launch_bounds__(kPdThreads, 1) paged_decode_cluster_kernel(con
     next += step;
     if (++st == S::kStages) st = 0;
   }
-  w.finish_sums();
+  w.finish(p, sp, b, rank * kPdWarps + warp, sp.nt, step);
   w.store_piece(pieces + warp * S::kPiece, lane);
   cp_async_wait<0>();
   __syncthreads();
