@@ -400,7 +400,8 @@ int lw_resid_rmsnorm_rows(void* x, const float* psum, const void* gamma, void* h
  * q_offsets [batch + 1] (device, q_offsets[0] = 0, never falling): rows
  * q_offsets[b] .. q_offsets[b + 1] - 1 are the newest tokens of sequence b, the
  * last of them at position kv_lens[b] - 1. Rows from q_offsets[batch] on belong
- * to no sequence: left as they were, or zeroed with zero_tail.
+ * to no sequence: left as they were, or zeroed with zero_tail. lw_paged_attention
+ * treats so the rows of a sequence that q_offsets lets run past `tokens` (recorded).
  *
  * Strides are in elements and multiples of 8; the last dimension is contiguous;
  * pointers are 16-byte aligned. dtype: LW_DTYPE_F16 or LW_DTYPE_BF16 of q, k,

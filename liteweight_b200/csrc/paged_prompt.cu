@@ -98,7 +98,7 @@ struct PromptParams {
 // A piece of work: up to 2 * rp positions of one sequence x one kv head's group,
 // against a slice of the key tiles they see.
 struct PromptWork {
-  int valid;           // 0: there is no more
+  int valid;           // 0: there is no more; -1: rows tok0 .. of a sequence that is refused (never published)
   int kvh, slice, slices, b;
   int tok0, np;        // first row of q, positions
   int pos0, last;      // position of the first, of the last
@@ -132,17 +132,19 @@ LW_DEV bool find_work(const PromptParams& p, int slot, int kvh, int slice, Promp
     hi = min(hi, lo + step);
   }
   const int i0 = (slot - (o / R + lo)) * R;
+  w.valid = 0;
   if (i0 < 0 || i0 >= n) return false;
+  w.tok0 = o + i0;
+  w.np = min(R, n - i0);
   if (o < 0 || (long long)o + n > p.T) {   // rows that q does not have
     lw_record_error(LW_ERR_BAD_INDEX);
+    w.valid = -1;
     return false;
   }
   w.valid = 1;
   w.kvh = kvh;
   w.slice = slice;
   w.b = lo;
-  w.tok0 = o + i0;
-  w.np = min(R, n - i0);
   w.pos0 = cut_len(p.c, len) - n + i0;   // negative: more rows than tokens
   if (w.pos0 < 0) lw_record_error(LW_ERR_BAD_INDEX);
   w.last = w.pos0 + w.np - 1;
@@ -486,7 +488,10 @@ __global__ void __launch_bounds__(kPmThreads, 1) paged_prompt_kernel(const __gri
       };
       while (more) {
         const int slot = slots - 1 - x / p.c.nkv, kvh = x % p.c.nkv, slice = z;
-        if (find_work(p, slot, kvh, slice, w) && !publish()) break;
+        const bool found = find_work(p, slot, kvh, slice, w);
+        // rows refused_0 .. of a sequence whose rows run past q's
+        const int refused = slice == 0 && w.valid < 0 ? min(w.np, p.T - w.tok0) : 0, refused_0 = w.tok0;
+        if (found && !publish()) break;
         if (lane == 0) {
           fence_proxy_async_smem();   // the answer before has been read
           mbar_arrive_expect_tx(smem_u32(&bar_clc), 16);
@@ -496,14 +501,20 @@ __global__ void __launch_bounds__(kPmThreads, 1) paged_prompt_kernel(const __gri
         if (!warp_wait(smem_u32(&bar_clc), asked++ & 1)) break;
         more = clc_answer(smem_u32(&clc_s), x, y, z);
         __syncwarp();
+        auto clear_row = [&](int r) {
+          for (int i = lane; i < p.group * (HD / 8); i += 32)
+            *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + r * p.o_t + (kvh * p.group + i / (HD / 8)) * p.o_h +
+                                      (i % (HD / 8)) * 8) = make_uint4(0, 0, 0, 0);
+        };
+        for (int r = max(0, refused_0); r < refused_0 + refused; ++r) {
+          if (p.zero_tail) clear_row(r);
+          if (p.slices > 1)   // nothing to join
+            for (int i = lane; i < p.group; i += 32) p.part_n[(long long)r * p.nq + kvh * p.group + i] = 1;
+        }
         if (p.zero_tail && slice == 0) {   // rows of no sequence: before the first, behind the last
           const int first = max(0, min(p.T, p.off[0])), behind = max(first, p.off[p.c.B]);
-          for (int x0 = slot; x0 < first + max(0, p.T - behind); x0 += slots) {
-            const int r = x0 < first ? x0 : behind + x0 - first;
-            for (int i = lane; i < p.group * (HD / 8); i += 32)
-              *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + r * p.o_t + (kvh * p.group + i / (HD / 8)) * p.o_h +
-                                        (i % (HD / 8)) * 8) = make_uint4(0, 0, 0, 0);
-          }
+          for (int x0 = slot; x0 < first + max(0, p.T - behind); x0 += slots)
+            clear_row(x0 < first ? x0 : behind + x0 - first);
         }
       }
       w.valid = 0;

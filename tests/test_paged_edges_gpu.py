@@ -205,3 +205,35 @@ def test_scores_of_minus_infinity_in_prompts(dtype, hd, window, sinks, width):
     assert (got == 0).all()
     with pytest.raises(Exception, match="out of range"):
         kernels.check_device_error()
+
+
+# ------------------------------------------------------------------ rows that are refused
+
+@pytest.mark.parametrize("width", [3, 5000])
+def test_rows_of_a_refused_sequence(width):
+    """A sequence whose rows run past q's is not computed; its rows in q are zero, or
+    as they were in a given `out`, with key slices (the wide table) and without.
+    What the allocator hands out is NaN and large numbers before the call."""
+    c = Batch([40, 30], 1, 64, 16, torch.float16)
+    wide = torch.full((2, width), -5, dtype=torch.int32, device=DEV)
+    wide[:, :3] = c.table[:, :3]
+    cache = (c.k_pages, c.v_pages, wide, c.kv_lens)
+    q = torch.randn(320, 2, 64, generator=gen(2), device=DEV).half()
+    for off, mine in (([0, 12, 400], slice(0, 12)), ([0, 12, 2 ** 31 - 1], slice(0, 12)),
+                      ([-5, 290, 320], slice(290, 320)), ([-300, 290, 320], slice(290, 320))):
+        counts = [b - a for a, b in zip(off, off[1:])]
+        b = 0 if mine.start == 0 else 1
+        want, tol = attend(q[mine], c.k[b], c.v[b], c.lens[b] - counts[b], None, 0, 0.125, torch.float16)
+        offs = torch.tensor(off, dtype=torch.int32, device=DEV)
+        theirs = torch.ones(320, dtype=torch.bool, device=DEV)
+        theirs[mine] = False
+        for given in (False, True):
+            for shape, dtype, value in (((320, 2, 64), torch.float16, float("nan")), ((1 << 24,), torch.int32, 7)):
+                left = [torch.full(shape, value, dtype=dtype, device=DEV) for _ in range(3)]
+                del left
+            out = torch.full_like(q, 3.0) if given else None
+            got = kernels.prompt_attention(q, *cache, offs, out=out)
+            with pytest.raises(Exception, match="out of range"):
+                kernels.check_device_error()
+            check(got[mine], want, tol)
+            assert (got[theirs] == (3 if given else 0)).all()
