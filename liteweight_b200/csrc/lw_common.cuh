@@ -212,10 +212,15 @@ LW_DEV void bulk_g2s(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar
 
 // Device error flag of this translation unit (each .cu file has its own copy:
 // the library is built without relocatable device code). Bounded waits that
-// give up record LW_ERR_TIMEOUT here; lw_take_device_error() reads them.
+// give up record LW_ERR_TIMEOUT here, paged-cache kernels LW_ERR_BAD_INDEX;
+// lw_take_device_error() reads them. The first is kept, but a timeout takes any
+// other's place: its launch left results unwritten, an index only skipped an access.
 static __device__ int lw_tu_error;
 
-LW_DEV void lw_record_error(int status) { atomicCAS(&lw_tu_error, 0, status); }
+LW_DEV void lw_record_error(int status) {
+  if (status == LW_ERR_TIMEOUT) atomicExch(&lw_tu_error, status);
+  else atomicCAS(&lw_tu_error, 0, status);
+}
 
 // Wait for phase `parity` of the mbarrier at `bar`, bounded by the global
 // timer (timeout_ns) and an iteration cap; records LW_ERR_TIMEOUT on giving up.

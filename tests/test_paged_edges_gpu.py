@@ -237,3 +237,27 @@ def test_rows_of_a_refused_sequence(width):
                 kernels.check_device_error()
             check(got[mine], want, tol)
             assert (got[theirs] == (3 if given else 0)).all()
+
+
+# ------------------------------------------------------------------ the error word
+
+def test_a_wait_that_gave_up_is_reported_before_an_index(tmp_path):
+    """A launch that records both has invalid results, whatever came first. The word
+    is the one every .cu file of the library has, here in a small library of its own."""
+    import ctypes
+    import subprocess
+
+    from liteweight_b200 import build
+    src = tmp_path / "word.cu"
+    src.write_text('#include "lw_common.cuh"\n'
+                   "__global__ void record(int a, int b) { if (a) lw::lw_record_error(a); if (b) lw::lw_record_error(b); }\n"
+                   'extern "C" int both(int a, int b) { record<<<1, 1>>>(a, b); return lw_tu_take_error(); }\n')
+    out = tmp_path / "libword.so"
+    subprocess.run([build.nvcc(), *build.ARCH, *build.FLAGS, "-shared", "-I", str(build.CSRC), str(src), "-o", str(out)],
+                   check=True, timeout=300)
+    lib = ctypes.CDLL(str(out))
+    timeout, index = 8, 9
+    for a, b, want in ((0, 0, 0), (index, 0, index), (timeout, 0, timeout), (timeout, index, timeout),
+                       (index, timeout, timeout), (index, index, index)):
+        assert lib.both(a, b) == want
+        assert lib.both(0, 0) == 0
