@@ -417,6 +417,8 @@ const char* lw_status_string(int status) {
 int lw_abi_version(void) { return 114; }
 
 int lw_take_device_error(void) {
+  // every stream's kernels: the copies below wait for the default stream's alone
+  if (cudaDeviceSynchronize() != cudaSuccess) return LW_ERR_LAUNCH;
   const int mine = lw_tu_take_error();
   const int dec = lw_decode_take_error();
   const int tp = lw_decode_tp_take_error();

@@ -261,3 +261,19 @@ def test_a_wait_that_gave_up_is_reported_before_an_index(tmp_path):
                        (index, timeout, timeout), (index, index, index)):
         assert lib.both(a, b) == want
         assert lib.both(0, 0) == 0
+
+
+def test_errors_of_calls_still_running_on_other_streams():
+    """check_device_error waits for them."""
+    c = Batch([100], 2, 64, 16, torch.float16)
+    q = torch.randn(1, 4, 64, generator=gen(2), device=DEV).half()
+    kernels.paged_attention(q, *c.cache())
+    c.table[0, 2] = 10 ** 6
+    torch.cuda.synchronize()
+    kernels.check_device_error()
+    with torch.cuda.stream(torch.cuda.Stream(DEV)):
+        torch.cuda._sleep(200_000_000)   # cycles: about 0.1 s
+        kernels.paged_attention(q, *c.cache())
+    with pytest.raises(Exception, match="out of range"):
+        kernels.check_device_error()
+    kernels.check_device_error()
