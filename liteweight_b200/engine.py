@@ -439,6 +439,18 @@ class PeerExchange:
 _TUNED: dict = {}   # DecodeEngine.tune_kernels' choices in this process
 
 
+def forget_tuning() -> None:
+    """Engines built after this call time their GEMV kernels anew (DecodeEngine.tune_kernels)."""
+    _TUNED.clear()
+
+
+def pick_kernel(times: dict[int, list[float]], margin: float) -> int:
+    """The ring (0), unless the register pipeline (1) is faster by more than
+    `margin`; by each one's least disturbed round, so that another stream's work
+    beside some of them does not decide."""
+    return 1 if min(times[1]) < min(times[0]) * (1.0 - margin) else 0
+
+
 class DecodeEngine:
     """Batched greedy decode of a Llama model on one GPU (or one tensor-parallel rank)."""
 
@@ -863,12 +875,12 @@ class DecodeEngine:
     def tune_kernels(self, reps: int = 5, margin: float = 0.03) -> dict:
         """Per projection class of the decode step (qkv, o, gu, down, lm_head),
         time its launches alone (a CUDA graph replayed `reps` times, CUDA
-        events) with the shared-memory ring GEMV and with the register-pipeline
-        GEMV, and keep the ring unless the other is faster by more than
-        `margin`. Runs on the engine's scratch state (before start()). A process
-        times a class of launches once: engines of the same shapes then run the
-        same kernels and give the same bits, where two timings of a close call
-        can differ."""
+        events, three rounds in turn) with the shared-memory ring GEMV and with
+        the register-pipeline GEMV, and keep the ring unless the other is faster
+        by more than `margin`. Runs on the engine's scratch state (before
+        start()). A process times a class of launches once: engines of the same
+        shapes then run the same kernels and give the same bits, where two timings
+        of a close call can differ; forget_tuning() drops the choices."""
         classes = []
         for kind, _a, n in self.calls:
             if kind == "gemv" and n not in classes:
@@ -884,7 +896,7 @@ class DecodeEngine:
                     if kind == "gemv" and n == name:
                         a.kernel = self.stat_args[id(a)].kernel = int(_TUNED[key]["kernel"] != "ring")
                 continue
-            ms = {}
+            times, graphs = {0: [], 1: []}, {}
             for kern in (0, 1):
                 for kind, a, n in self.calls:
                     if kind == "gemv" and n == name:
@@ -900,21 +912,24 @@ class DecodeEngine:
                     self.enqueue_only(name)
                 g.replay()
                 torch.cuda.synchronize(dev)
+                graphs[kern] = g
+            for kern in (0, 1) * 3:
                 e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
                 e0.record()
                 for _ in range(reps):
-                    g.replay()
+                    graphs[kern].replay()
                 e1.record()
                 torch.cuda.synchronize(dev)
-                ms[kern] = e0.elapsed_time(e1) / reps
-                del g
-            pick = 1 if ms[1] < ms[0] * (1.0 - margin) else 0
+                times[kern].append(e0.elapsed_time(e1) / reps)
+            del g, graphs
+            pick = pick_kernel(times, margin)
             for kind, a, n in self.calls:
                 if kind == "gemv" and n == name:
                     a.kernel = pick
                     self.stat_args[id(a)].kernel = pick
             self.kernel_choice[name] = {"kernel": "ring" if pick == 0 else "register-pipeline",
-                                        "ring_us": round(ms[0] * 1e3, 2), "pipeline_us": round(ms[1] * 1e3, 2)}
+                                        "ring_us": round(min(times[0]) * 1e3, 2),
+                                        "pipeline_us": round(min(times[1]) * 1e3, 2)}
             _TUNED[key] = dict(self.kernel_choice[name])
         self.check()
         return self.kernel_choice

@@ -108,3 +108,16 @@ def test_tc_supported_per_rank_shards():
     assert all(E.tc_supported(spec, tp) for tp in (1, 2, 4, 8))
     odd = E.LlamaSpec(**{**E.LLAMA_3_8B, "inter": 14336 + 32}, bits=4, group_size=128)
     assert not E.tc_supported(odd, 1)
+
+
+def test_kernel_choice_goes_by_the_least_disturbed_round():
+    assert E.pick_kernel({0: [13.4, 60.0, 13.8], 1: [15.0, 15.2, 15.1]}, 0.03) == 0   # a round beside other work
+    assert E.pick_kernel({0: [60.0, 61.0, 13.4], 1: [15.0, 15.2, 15.1]}, 0.03) == 0
+    assert E.pick_kernel({0: [10.0] * 3, 1: [9.8, 9.8, 9.8]}, 0.03) == 0               # within the margin
+    assert E.pick_kernel({0: [10.0] * 3, 1: [12.0, 9.0, 30.0]}, 0.03) == 1
+
+
+def test_tuning_can_be_forgotten():
+    E._TUNED[("a class",)] = {"kernel": "ring"}
+    E.forget_tuning()
+    assert not E._TUNED
