@@ -191,7 +191,8 @@ __device__ __noinline__ void add_nonfinite(const PromptParams& p, const PromptWo
     tmem_ld8(to + 8 * x, o);
     for (int i = 0; i < w.nt; ++i) {
       const int key0 = w.key_of(i);
-      if (!(key0 + kPmKeys - 1 > w.pos0 || (p.window > 0 && key0 <= w.last - p.window))) continue;
+      if (!(key0 + kPmKeys - 1 > w.pos0 || (p.window > 0 && key0 <= w.last - p.window && key0 + kPmKeys > sinks)))
+        continue;   // every row sees the tile whole
       for (int key = key0; key < key0 + kPmKeys; ++key) {
         if (!(key <= pos && (key > lo || key < sinks))) continue;
         const int page = page_id(p.c, w.b, key);
@@ -543,7 +544,8 @@ __global__ void __launch_bounds__(kPmThreads, 1) paged_prompt_kernel(const __gri
       const int lo = windowed ? pos - p.window : -1;   // keys above lo, or below sinks
       const int sinks = windowed ? p.sinks : 0;
       float m = -INFINITY, l = 0.f;
-      // key tiles that a row of this row tile / of the piece does not see whole
+      // key tiles that a row of this row tile / of the piece does not see whole:
+      // past the one, or up to the other and not among the first keys alone
       const int mask_hi = first_pos - (kPmKeys - 1), mask_lo = windowed ? last_pos - p.window : -1;
       const int cut_hi = w.pos0 - (kPmKeys - 1), cut_lo = windowed ? w.last - p.window : -1;
       int key0 = w.key_of(0);
@@ -557,7 +559,8 @@ __global__ void __launch_bounds__(kPmThreads, 1) paged_prompt_kernel(const __gri
 #pragma unroll
         for (int x = 0; x < 4; ++x) tmem_regs_ready(s[x]);
         const uint32_t lost = lost_s[tiles & 7];
-        if (key0 > mask_hi || key0 <= mask_lo || lost) {
+        const bool past_sinks = key0 + kPmKeys > sinks;
+        if (key0 > mask_hi || (key0 <= mask_lo && past_sinks) || lost) {
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             // bit e: the row sees key k0 + e
@@ -600,7 +603,7 @@ __global__ void __launch_bounds__(kPmThreads, 1) paged_prompt_kernel(const __gri
             }
           }
         }
-        if (g == 0 && (key0 > cut_hi || key0 <= cut_lo)) {
+        if (g == 0 && (key0 > cut_hi || (key0 <= cut_lo && past_sinks))) {
           // row r of V
           const int xv = 2 * tiles + 1;
           if (!(ok = warp_wait(smem_u32(&bar_full[xv % NS]), (xv / NS) & 1))) break;

@@ -277,3 +277,70 @@ def test_errors_of_calls_still_running_on_other_streams():
     with pytest.raises(Exception, match="out of range"):
         kernels.check_device_error()
     kernels.check_device_error()
+
+
+# ------------------------------------------------------------------ many first keys beside a window
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("sinks", [128, 130, 512, 1000, 1900])
+@pytest.mark.parametrize("new", [77, 2000])
+def test_sinks_that_fill_tiles(dtype, hd, sinks, new):
+    """First keys that every row sees, those that part of the rows' windows reach,
+    and what an infinity in the one or the other gives."""
+    n, window, group = 2000, 90, 5
+    c = Batch([n], 1, hd, 32, dtype)
+    q = torch.randn(new, group, hd, generator=gen(6), device=DEV).to(dtype)
+    first = n - new
+    want, tol = attend(q, c.k[0], c.v[0], first, window, sinks, hd ** -0.5, dtype)
+    check(kernels.prompt_attention(q, *c.cache(), offsets(new), window=window, sinks=sinks), want, tol)
+    p = torch.arange(first, n, device=DEV)
+    dims = torch.arange(hd, device=DEV) != 5
+    for key in (0, 127, sinks - 1, sinks, n - 60, n - 1):
+        v = c.v[0].clone()
+        v[key, 0, 5] = float("inf")
+        c.put(0, 0, c.k[0], v)
+        got = kernels.prompt_attention(q, *c.cache(), offsets(new), window=window, sinks=sinks)
+        seen = (p >= key) & ((p - key < window) | (key < sinks))
+        assert (got[seen][:, :, 5] == float("inf")).all()
+        check(got[~seen], want[~seen], tol[~seen])
+        check(got[:, :, dims], want[:, :, dims], tol[:, :, dims])
+        c.put(0, 0, c.k[0], c.v[0])
+    kernels.check_device_error()
+
+
+def test_an_infinity_beside_many_sinks_costs_what_it_costs_beside_few():
+    """Only tiles that part of the rows see are searched for it: walking all first
+    keys took 46 times as long for 16384 of them as for 256, and past some 340000 a row
+    tile's walk would outlast the other warps' bounded waits."""
+    hd, new, batch, window = 128, 128, 10, 100
+    took = []
+    for sinks in (256, 16384):
+        n = sinks + 512
+        c = Batch([n], 8, hd, 64, torch.float16)
+        v = c.v[0].clone()
+        v[n - 5, :, 3] = float("inf")
+        c.put(0, 0, c.k[0], v)
+        table = c.table[:, :-(-n // 64)].expand(batch, -1).contiguous()   # the same pages for all
+        lens = c.kv_lens.expand(batch).contiguous()
+        q = torch.randn(new * batch, 16, hd, generator=gen(1), device=DEV).half()
+        call = lambda: kernels.prompt_attention(q, c.k_pages, c.v_pages, table, lens, offsets(*[new] * batch),  # noqa: E731
+                                                window=window, sinks=sinks)
+        got = call()
+        want, tol = attend(q[:new], c.k[0], c.v[0], n - new, window, sinks, hd ** -0.5, torch.float16)
+        dims = torch.arange(hd, device=DEV) != 3
+        check(got[:new, :, dims], want[:, :, dims], tol[:, :, dims])
+        seen = torch.arange(n - new, n, device=DEV) >= n - 5
+        assert (got[:new][seen][:, :, 3] == float("inf")).all()
+        check(got[:new][~seen], want[~seen], tol[~seen])
+        times = []
+        for _ in range(3):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            call()
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        took.append(min(times))
+    kernels.check_device_error()
+    assert took[1] < 5 * took[0], took
