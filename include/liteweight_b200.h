@@ -47,7 +47,8 @@ typedef enum {
 /* Human-readable name of a status code (static string). */
 const char* lw_status_string(int status);
 
-/* ABI version of this library (major * 100 + minor). */
+/* ABI version of this header, and of a library (major * 100 + minor). */
+#define LW_ABI_VERSION 114
 int lw_abi_version(void);
 
 /* Number of CUDA kernels this library has enqueued since it was loaded

@@ -95,7 +95,8 @@ def lib() -> ctypes.CDLL:
 
 def bind():
     """The extension module over the paged-cache entry points (csrc/bind_paged.cpp),
-    loaded once; its calls go to lib()'s functions."""
+    loaded once; its calls go to lib()'s functions, which have to be of the version
+    and structs that it was built for."""
     global _bind
     if _bind is None:
         handle = lib()
@@ -107,7 +108,8 @@ def bind():
                                                                                        loader=loader))
         loader.exec_module(module)
         module.init(*(ctypes.cast(getattr(handle, f), c_void_p).value for f in
-                      ("lw_qk_norm_rope", "lw_paged_attention", "lw_paged_attention_workspace_size")))
+                      ("lw_abi_version", "lw_struct_size", "lw_qk_norm_rope", "lw_paged_attention",
+                       "lw_paged_attention_workspace_size")))
         _bind = module
     return _bind
 

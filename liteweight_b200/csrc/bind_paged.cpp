@@ -256,10 +256,19 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// init(address of lw_qk_norm_rope, of lw_paged_attention, of lw_paged_attention_workspace_size)
-PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n) {
+// init(address of lw_abi_version, of lw_struct_size, of lw_qk_norm_rope, of lw_paged_attention,
+// of lw_paged_attention_workspace_size). Refuses a library of another version or with other structs.
+PyObject* init(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    require(n == 3, "init: 3 addresses");
+    require(n == 5, "init: 5 addresses");
+    const int version = reinterpret_cast<decltype(&lw_abi_version)>(whole(args[0], "address"))();
+    const auto size = reinterpret_cast<decltype(&lw_struct_size)>(whole(args[1], "address"));
+    if (version != LW_ABI_VERSION || size(5) != sizeof(lw_paged_cache) || size(6) != sizeof(lw_qk_norm_rope_args) ||
+        size(7) != sizeof(lw_paged_attention_args))
+      throw Refused{PyExc_RuntimeError, "lw_bind.so was built for version " + std::to_string(LW_ABI_VERSION) +
+                                            " of the library and got version " + std::to_string(version) +
+                                            " or other structs; build both with `python -m liteweight_b200.build`"};
+    PyObject* const* a = args + 2;
     g_rope = reinterpret_cast<decltype(g_rope)>(whole(a[0], "address"));
     g_attention = reinterpret_cast<decltype(g_attention)>(whole(a[1], "address"));
     g_workspace = reinterpret_cast<decltype(g_workspace)>(whole(a[2], "address"));

@@ -414,7 +414,7 @@ const char* lw_status_string(int status) {
   }
 }
 
-int lw_abi_version(void) { return 114; }
+int lw_abi_version(void) { return LW_ABI_VERSION; }
 
 int lw_take_device_error(void) {
   // every stream's kernels: the copies below wait for the default stream's alone

@@ -161,3 +161,38 @@ def test_rope_asserts():
                dict(q_offsets=torch.zeros(2, dtype=torch.int32))):
         with pytest.raises(AssertionError):
             kernels.qk_norm_rope(**{**good, **kw})
+
+
+STUB_USE = """
+from liteweight_b200 import _native as nat
+import liteweight_b200.engine
+try:
+    nat.bind()
+    print("bound")
+except RuntimeError as e:
+    print("refused:", e)
+"""
+
+
+@pytest.mark.parametrize("abi,grow,want", [(0, 0, "bound"), (1, 0, "refused"), (-1, 0, "refused"), (0, 8, "refused")])
+def test_the_extension_module_takes_only_the_library_it_was_built_for(lib, tmp_path, abi, grow, want):
+    """Against a stand-in library whose version, or one of whose structs, differs."""
+    import os
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    import liteweight_b200.engine  # noqa: F401  (registers the engine entry points)
+    sizes = [lib.lw_struct_size(i) for i in range(8)]
+    sizes[7] += grow
+    src = tmp_path / "stub.c"
+    src.write_text("".join(f"long {f}() {{ return 0; }}\n" for f in nat.declared_symbols()
+                           if f not in ("lw_abi_version", "lw_struct_size")) +
+                   f"int lw_abi_version(void) {{ return {lib.lw_abi_version() + abi}; }}\n"
+                   f"unsigned long lw_struct_size(int i) {{ static unsigned long s[] = {{{', '.join(map(str, sizes))}}};"
+                   " return s[i]; }\n")
+    out = tmp_path / "stub.so"
+    subprocess.run(["gcc", "-shared", "-fPIC", "-o", str(out), str(src)], check=True)
+    got = subprocess.run([sys.executable, "-c", STUB_USE], env={**os.environ, "LW_B200_LIB": str(out)}, text=True,
+                         capture_output=True, timeout=300, cwd=Path(__file__).resolve().parent.parent)
+    assert got.stdout.startswith(want), got.stdout + got.stderr
