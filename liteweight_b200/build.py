@@ -7,7 +7,9 @@ The library is a plain C-ABI shared object (include/liteweight_b200.h) with
 the CUDA runtime linked statically, loaded from Python with ctypes. nvcc
 cross-compiles for sm_100a without a GPU. lw_bind.so is a Python extension module
 over that ABI for the calls whose argument handling in Python would cost more
-than their launches; it is built by g++ against torch's headers.
+than their launches; it is built by g++ against torch's headers. The C library
+alone needs neither torch nor Python's headers: `python liteweight_b200/build.py`
+links it before it reports that the extension module could not be built.
 """
 
 from __future__ import annotations
@@ -18,6 +20,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -28,6 +31,7 @@ LIB = LIB_DIR / "liblw_b200.so"
 BIND_SRC = CSRC / "bind_paged.cpp"
 BIND = LIB_DIR / "lw_bind.so"
 STAMP = LIB_DIR / "liblw_b200.sha"
+BIND_STAMP = LIB_DIR / "lw_bind.sha"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-O3", "--expt-relaxed-constexpr",
@@ -41,12 +45,20 @@ def sources() -> list[Path]:
 
 def _digest() -> str:
     h = hashlib.sha256()
-    for f in sorted(list(CSRC.glob("*.cu")) + list(CSRC.glob("*.cuh")) + list(INCLUDE.glob("*.h")) + [BIND_SRC]):
+    for f in sorted(list(CSRC.glob("*.cu")) + list(CSRC.glob("*.cuh")) + list(INCLUDE.glob("*.h"))):
         h.update(f.name.encode())
         h.update(f.read_bytes())
-    # the extension module is tied to this interpreter and torch
+    h.update(" ".join(ARCH + FLAGS).encode())
+    return h.hexdigest()
+
+
+def _bind_digest() -> str:
+    """The extension module is tied to this interpreter and torch."""
     import torch
-    h.update(" ".join(ARCH + FLAGS + BIND_FLAGS + [sys.version, torch.__version__]).encode())
+    h = hashlib.sha256()
+    for f in [BIND_SRC, *sorted(INCLUDE.glob("*.h"))]:
+        h.update(f.read_bytes())
+    h.update(" ".join(BIND_FLAGS + [sys.version, torch.__version__]).encode())
     return h.hexdigest()
 
 
@@ -68,19 +80,28 @@ def nvcc() -> str:
     raise RuntimeError("nvcc not found: the liteweight_b200 CUDA library cannot be built")
 
 
+def _current(out: Path, stamp: Path, digest) -> bool:
+    return out.exists() and stamp.exists() and stamp.read_text().strip() == digest()
+
+
+def _library_current() -> bool:
+    return _current(LIB, STAMP, _digest)
+
+
+def _bind_current() -> bool:
+    try:
+        return _current(BIND, BIND_STAMP, _bind_digest)
+    except ImportError:
+        return False
+
+
 def up_to_date() -> bool:
-    return LIB.exists() and BIND.exists() and STAMP.exists() and STAMP.read_text().strip() == _digest()
+    return _library_current() and _bind_current()
 
 
-def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile every csrc/*.cu for sm_100a, link liblw_b200.so and build lw_bind.so
-    (skipped when up to date)."""
-    if not force and up_to_date():
-        return LIB
-    LIB_DIR.mkdir(exist_ok=True)
+def _build_library(cc: str, verbose: bool) -> None:
     obj_dir = LIB_DIR / "obj"
     obj_dir.mkdir(exist_ok=True)
-    cc = nvcc()
     objs, procs = [], []
     for src in sources():
         obj = obj_dir / (src.stem + ".o")
@@ -89,11 +110,6 @@ def build(force: bool = False, verbose: bool = False) -> Path:
             print(" ".join(cmd), flush=True)
         procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
         objs.append(obj)
-    bind_tmp = BIND.with_suffix(".so.tmp")
-    cmd = _bind_command(bind_tmp)
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    procs.append((BIND_SRC, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
     failed = []
     for src, p in procs:
         out, _ = p.communicate()
@@ -102,15 +118,46 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         elif verbose and out:
             print(out.decode(errors="replace"))
     if failed:
-        raise RuntimeError("the build failed\n" + "\n".join(failed))
+        raise RuntimeError("nvcc failed\n" + "\n".join(failed))
     tmp = LIB.with_suffix(".so.tmp")
     cmd = [cc, *ARCH, "-shared", "-cudart", "static", "-o", str(tmp), *map(str, objs), "-lrt", "-ldl", "-lpthread"]
     if verbose:
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)
     os.replace(tmp, LIB)
-    os.replace(bind_tmp, BIND)
     STAMP.write_text(_digest())
+
+
+def _build_bind(verbose: bool) -> None:
+    tmp = BIND.with_suffix(".so.tmp")
+    try:
+        cmd = _bind_command(tmp)
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        made = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)
+        why = made.stdout.decode(errors="replace") if made.returncode else None
+    except (ImportError, AttributeError, OSError) as e:   # no torch, none that it can be built with, no compiler
+        why = f"{type(e).__name__}: {e}"
+    if why is not None:
+        raise RuntimeError(f"{BIND_SRC.name}, the Python extension module, could not be built:\n{why}")
+    os.replace(tmp, BIND)
+    BIND_STAMP.write_text(_bind_digest())
+
+
+def build(force: bool = False, verbose: bool = False) -> Path:
+    """Compile every csrc/*.cu for sm_100a, link liblw_b200.so and build lw_bind.so
+    (each skipped when up to date). The C library needs neither torch nor Python:
+    it is there when only the extension module fails."""
+    if not force and up_to_date():
+        return LIB
+    LIB_DIR.mkdir(exist_ok=True)
+    # side by side; the C library's failure is the one that is raised
+    with ThreadPoolExecutor(1) as pool:
+        bind = None if not force and _bind_current() else pool.submit(_build_bind, verbose)
+        if force or not _library_current():
+            _build_library(nvcc(), verbose)
+        if bind is not None:
+            bind.result()
     return LIB
 
 

@@ -196,3 +196,32 @@ def test_the_extension_module_takes_only_the_library_it_was_built_for(lib, tmp_p
     got = subprocess.run([sys.executable, "-c", STUB_USE], env={**os.environ, "LW_B200_LIB": str(out)}, text=True,
                          capture_output=True, timeout=300, cwd=Path(__file__).resolve().parent.parent)
     assert got.stdout.startswith(want), got.stdout + got.stderr
+
+
+def test_the_c_library_is_built_without_the_extension_module(tmp_path, monkeypatch):
+    """A compiler or a torch that the Python module cannot be built with does not cost
+    the C library, which needs neither; what failed is still raised, and built next time."""
+    (tmp_path / "csrc").mkdir()
+    src = tmp_path / "csrc" / "one.cu"
+    src.write_text('extern "C" int lw_one(void) { return 1; }\n')
+    monkeypatch.setattr(lwbuild, "CSRC", tmp_path / "csrc")
+    monkeypatch.setattr(lwbuild, "LIB_DIR", tmp_path / "lib")
+    for name, file in (("LIB", "liblw_b200.so"), ("BIND", "lw_bind.so"), ("STAMP", "liblw_b200.sha"),
+                       ("BIND_STAMP", "lw_bind.sha")):
+        monkeypatch.setattr(lwbuild, name, tmp_path / "lib" / file, raising=False)
+
+    def no_torch(out):
+        raise ImportError("no torch")
+
+    for command in (lambda out: ["false"], no_torch, lambda out: ["/nonexistent/g++"]):
+        monkeypatch.setattr(lwbuild, "_bind_command", command)
+        lwbuild.LIB.unlink(missing_ok=True)
+        with pytest.raises(RuntimeError, match="bind_paged.cpp"):
+            lwbuild.build()
+        assert ctypes.CDLL(str(lwbuild.LIB)).lw_one() == 1
+        assert not lwbuild.BIND.exists() and not lwbuild.up_to_date()
+    made = lwbuild.LIB.stat().st_mtime_ns
+    monkeypatch.setattr(lwbuild, "_bind_command", lambda out: ["cp", str(src), str(out)])
+    lwbuild.build()
+    assert lwbuild.BIND.exists() and lwbuild.up_to_date()
+    assert lwbuild.LIB.stat().st_mtime_ns == made   # not built again
