@@ -52,6 +52,7 @@
 // is waited for did not shorten it (526 -> 575 us): the bound is what two softmax
 // warps per scheduler get through. Four (two threads per row) were slower (685).
 #include <algorithm>
+#include <cmath>
 
 #include "paged.cuh"
 #include "tcgen05.cuh"
@@ -797,7 +798,8 @@ int check(const lw_paged_attention_args* a) {
   int st = lw_host::check_cache(a->cache);
   if (st) return st;
   if (a->tokens < 0 || a->n_q_heads <= 0 || a->n_q_heads % a->cache.n_kv_heads || a->sinks < 0) return LW_ERR_BAD_SHAPE;
-  if (!(a->scale > 0.f) || a->scale > 3.0e38f) return LW_ERR_BAD_SHAPE;   // the maximum is taken before scaling
+  // above 0: the maximum is taken before scaling; finite times log2(e), as the kernels use it
+  if (!(a->scale > 0.f) || !std::isfinite(a->scale * 1.4426950408889634f)) return LW_ERR_BAD_SHAPE;
   if (!a->q_offsets && a->tokens != a->cache.batch) return LW_ERR_BAD_SHAPE;
   if (a->q_offsets && a->n_q_heads / a->cache.n_kv_heads > 64) return LW_ERR_UNSUPPORTED;
   if (a->tokens == 0) return LW_OK;

@@ -225,3 +225,9 @@ def test_the_c_library_is_built_without_the_extension_module(tmp_path, monkeypat
     lwbuild.build()
     assert lwbuild.BIND.exists() and lwbuild.up_to_date()
     assert lwbuild.LIB.stat().st_mtime_ns == made   # not built again
+
+
+def test_scales_are_finite_times_log2_e(lib):
+    """The kernels' exponentials are of base 2: a scale that log2(e) takes past fp32 is refused too."""
+    for scale, status in ((3.4e38, 2), (3.0e38, 2), (2.4e38, 2), (2.3e38, 1)):   # 1: goes on to q's pointer
+        assert lib.lw_paged_attention(ctypes.byref(attn_args(scale=scale, q=None)), None) == status
