@@ -78,6 +78,9 @@ void same_device(std::initializer_list<const at::Tensor*> ts) {
   for (const at::Tensor* t : ts) require(!t->defined() || t->device() == dev, "all tensors must be on one device");
 }
 
+// The stride of a dimension; of one element (or none) it addresses nothing and may be any.
+long long stride_of(const at::Tensor& t, int dim) { return t.size(dim) > 1 ? t.stride(dim) : 0; }
+
 lw_paged_cache cache(const at::Tensor& k, const at::Tensor& v, const at::Tensor& table, const at::Tensor& lens) {
   lw_paged_cache c = {};
   const auto dt = k.scalar_type();
@@ -94,8 +97,10 @@ lw_paged_cache cache(const at::Tensor& k, const at::Tensor& v, const at::Tensor&
     require(n <= INT_MAX, "sizes past 2^31 - 1 are not supported");
   c.k_pages = k.data_ptr();
   c.v_pages = v.data_ptr();
-  c.k_strides[0] = k.stride(0), c.k_strides[1] = k.stride(1), c.k_strides[2] = k.stride(2);
-  c.v_strides[0] = v.stride(0), c.v_strides[1] = v.stride(1), c.v_strides[2] = v.stride(2);
+  for (int i = 0; i < 3; ++i) {
+    c.k_strides[i] = stride_of(k, i);
+    c.v_strides[i] = stride_of(v, i);
+  }
   c.n_pages = (int)k.size(0);
   c.n_kv_heads = (int)k.size(1);
   c.page_size = (int)k.size(2);
@@ -103,7 +108,7 @@ lw_paged_cache cache(const at::Tensor& k, const at::Tensor& v, const at::Tensor&
   c.dtype = dt == at::kHalf ? LW_DTYPE_F16 : LW_DTYPE_BF16;
   c.batch = (int)table.size(0);
   c.page_table = static_cast<const int*>(table.data_ptr());
-  c.table_stride = table.stride(0);
+  c.table_stride = stride_of(table, 0);
   c.table_width = (int)table.size(1);
   c.kv_lens = static_cast<const int*>(lens.data_ptr());
   return c;
@@ -114,8 +119,8 @@ void rows(const at::Tensor& t, const at::Tensor& like, long long (&strides)[2], 
   require(t.scalar_type() == like.scalar_type() && t.dim() == 3 && t.size(2) == like.size(3) &&
               (t.stride(2) == 1 || t.numel() == 0) && t.size(0) <= INT_MAX && t.size(1) <= INT_MAX,
           why);
-  strides[0] = t.stride(0);
-  strides[1] = t.stride(1);
+  strides[0] = stride_of(t, 0);
+  strides[1] = stride_of(t, 1);
 }
 
 const int* offsets(const at::Tensor& off, int batch, int64_t tokens) {
@@ -123,7 +128,8 @@ const int* offsets(const at::Tensor& off, int batch, int64_t tokens) {
     require(tokens == batch, "one new token per sequence: as many rows as sequences");
     return nullptr;
   }
-  require(off.scalar_type() == at::kInt && off.dim() == 1 && off.size(0) == (int64_t)batch + 1 && off.stride(0) == 1,
+  require(off.scalar_type() == at::kInt && off.dim() == 1 && off.size(0) == (int64_t)batch + 1 &&
+              (off.stride(0) == 1 || off.size(0) <= 1),
           "q_offsets: int32 [batch + 1], contiguous");
   return static_cast<const int*>(off.data_ptr());
 }
@@ -172,7 +178,8 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
     require(cos.dim() == 2 && cos.size(1) == hd && sin.sizes() == cos.sizes(), "cos / sin: [positions, head_dim]");
     require((cos.scalar_type() == dt || cos.scalar_type() == at::kFloat) && sin.scalar_type() == cos.scalar_type(),
             "cos / sin: float32 or the cache's type");
-    require(cos.strides() == sin.strides() && (cos.stride(1) == 1 || cos.numel() == 0) && cos.size(0) <= INT_MAX,
+    require(stride_of(cos, 0) == stride_of(sin, 0) && ((cos.stride(1) == 1 && sin.stride(1) == 1) || cos.numel() == 0) &&
+                cos.size(0) <= INT_MAX,
             "cos / sin: rows contiguous, strides alike");
     require(qw.defined() == kw.defined(), "norm weights for both queries and keys, or for neither");
     for (const at::Tensor* w : {&qw, &kw})
@@ -197,7 +204,7 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
     p.n_q_heads = (int)q.size(1);
     p.rope_cos = cos.data_ptr();
     p.rope_sin = sin.data_ptr();
-    p.rope_stride = cos.stride(0);
+    p.rope_stride = stride_of(cos, 0);
     p.rope_dtype = cos.scalar_type() == at::kFloat ? LW_DTYPE_F32 : p.cache.dtype;
     p.rope_rows = (int)cos.size(0);
     p.q_weight = qw.defined() ? qw.data_ptr() : nullptr;

@@ -344,3 +344,40 @@ def test_an_infinity_beside_many_sinks_costs_what_it_costs_beside_few():
         took.append(min(times))
     kernels.check_device_error()
     assert took[1] < 5 * took[0], took
+
+
+# ------------------------------------------------------------------ layouts
+
+def test_strides_of_dimensions_of_one_element():
+    """They address nothing, so any will do: one token, one kv head, one page, one position."""
+    hd = 64
+
+    def odd(x, *dims):   # the same tensor, with strides of 3 for these dimensions of one element
+        assert all(x.shape[d] == 1 for d in dims)
+        return x.as_strided(x.shape, [3 if d in dims else s for d, s in enumerate(x.stride())])
+
+    pools = [torch.randn(1, 1, 16, hd, generator=gen(i), device=DEV).half() for i in range(2)]
+    table = torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    lens = torch.ones(1, dtype=torch.int32, device=DEV)
+    off = offsets(1)
+    q, k, v = (torch.randn(1, n, hd, generator=gen(9), device=DEV).half() for n in (4, 1, 1))
+    cos, sin = (torch.randn(1, hd, generator=gen(i), device=DEV) for i in range(2))
+    results = []
+    for make in (lambda x, *dims: x.clone(), odd):
+        kp, vp = (make(x.clone(), 0, 1) for x in pools)
+        out = make(torch.zeros(1, 4, hd, device=DEV).half(), 0)
+        got = kernels.qk_norm_rope(make(q, 0), make(k, 0, 1), make(v, 0, 1), make(cos, 0), make(sin, 0), kp, vp, table,
+                                   lens, out=out)
+        lens += 5
+        one = kernels.paged_attention(make(got, 0), kp, vp, table, lens)
+        all_of_it = kernels.prompt_attention(make(got, 0), kp, vp, table, lens, off, out=make(torch.zeros_like(q), 0))
+        lens -= 5
+        results.append([got, kp, vp, one, all_of_it])
+    # cos a row of a wide tensor, sin one of a narrow one
+    wide = torch.cat([cos, cos], dim=1)[:, :hd]
+    kp, vp = (x.clone() for x in pools)
+    results.append([kernels.qk_norm_rope(q, k, v, wide, sin, kp, vp, table, lens), kp, vp])
+    kernels.check_device_error()
+    for other in results[1:]:
+        for a, b in zip(results[0], other):
+            assert torch.equal(a, b)
