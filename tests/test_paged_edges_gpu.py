@@ -381,3 +381,184 @@ def test_strides_of_dimensions_of_one_element():
     for other in results[1:]:
         for a, b in zip(results[0], other):
             assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------ launches of more work than the GPU takes at once
+
+def prompt_blocks(rows, group, nkv, batch):
+    """Blocks of a prompt_attention launch without key slices: 2 * (128 // group) positions each."""
+    return (rows // (2 * (128 // group)) + batch) * nkv
+
+
+# ragged, with sequences of no and of one new token, cached prefixes, and a last row tile that is not full
+MANY = ([1, 700, 0, 333, 64, 0, 1, 415, 37], [0, 150, 9, 1000, 64, 40, 700, 0, 3])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("nkv,group", [(2, 48), (2, 64), (3, 33)])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (130, 0), (70, 5)])
+def test_blocks_take_over_the_work_of_others(dtype, hd, nkv, group, window, sinks):
+    """Several pieces per CTA: rows of one and of two row tiles, of few and of many key
+    tiles follow one another in the same barriers, ring slots and tensor memory."""
+    new, before = MANY
+    lens = [a + b for a, b in zip(new, before)]
+    assert prompt_blocks(sum(new), group, nkv, len(new)) > 2 * torch.cuda.get_device_properties(0).multi_processor_count
+    c = Batch(lens, nkv, hd, 16, dtype, seed=group)
+    off = offsets(*new)
+    q = (torch.randn(sum(new), nkv * group, hd, generator=gen(3), device=DEV) * 1.7).to(dtype)
+    got = kernels.prompt_attention(q, *c.cache(), off, window=window, sinks=sinks)
+    kernels.check_device_error()
+    at = 0
+    for b, n in enumerate(new):
+        rows = slice(at, at + n)
+        at += n
+        if n:
+            check(got[rows], *attend(q[rows], c.k[b], c.v[b], before[b], window, sinks, hd ** -0.5, dtype))
+    for _ in range(3):
+        assert torch.equal(kernels.prompt_attention(q, *c.cache(), off, window=window, sinks=sinks), got)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (100, 3)])
+def test_an_infinity_of_one_piece_stays_out_of_the_next(hd, window, sinks):
+    """A CTA's piece whose values were searched and mended, then pieces that do not see the infinity."""
+    n, nkv, group, dtype = 900, 2, 48, torch.bfloat16
+    lens = [n, 200, 300]
+    assert prompt_blocks(sum(lens), group, nkv, 3) > 2 * torch.cuda.get_device_properties(0).multi_processor_count
+    c = Batch(lens, nkv, hd, 32, dtype)
+    q = torch.randn(sum(lens), nkv * group, hd, generator=gen(3), device=DEV).to(dtype)
+    off = offsets(*lens)
+    clean = kernels.prompt_attention(q, *c.cache(), off, window=window, sinks=sinks)
+    p = torch.arange(n, device=DEV)
+    for key in (0, 450, 801):
+        v = c.v[0].clone()
+        v[key, 1, 5] = float("inf")
+        c.put(0, 0, c.k[0], v)
+        got = kernels.prompt_attention(q, *c.cache(), off, window=window, sinks=sinks)
+        seen = (p >= key) & ((p - key < window) | (key < sinks) if window else True)
+        assert (got[:n][seen][:, group:, 5] == float("inf")).all()
+        want, tol = attend(q[:n], c.k[0], c.v[0], 0, window, sinks, hd ** -0.5, dtype)
+        check(got[:n][~seen], want[~seen], tol[~seen])
+        check(got[:n, :group], want[:, :group], tol[:, :group])
+        dims = torch.arange(hd, device=DEV) != 5
+        check(got[:n][:, :, dims], want[:, :, dims], tol[:, :, dims])
+        assert torch.equal(got[n:], clean[n:])   # sequences that do not hold the key
+        c.put(0, 0, c.k[0], c.v[0])
+    kernels.check_device_error()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hd,nkv,group", [(64, 2, 4), (128, 1, 8), (128, 2, 12)])
+@pytest.mark.parametrize("lens,window,sinks", [
+    ([131071], None, 0), ([40001, 3, 90000, 0], None, 0), ([131071, 70000], 60000, 5000)])
+def test_decode_over_long_contexts(dtype, hd, nkv, group, lens, window, sinks):
+    """One item spans dozens of CTAs, whose pieces the second kernel joins."""
+    c = Batch(lens, nkv, hd, 64, dtype, seed=hd)
+    q = (torch.randn(len(lens), nkv * group, hd, generator=gen(7), device=DEV) * 1.7).to(dtype)
+    got = kernels.paged_attention(q, *c.cache(), window=window, sinks=sinks)
+    kernels.check_device_error()
+    for b, n in enumerate(lens):
+        check(got[b:b + 1], *attend(q[b:b + 1], c.k[b], c.v[b], n - 1, window, sinks, hd ** -0.5, dtype))
+    assert torch.equal(kernels.paged_attention(q, *c.cache(), window=window, sinks=sinks), got)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_prompts_over_long_contexts(dtype):
+    """A chunk far into its context, with key slices (few rows) and without (a batch of them)."""
+    lens, new = [70001, 5, 66000], [20, 5, 40]
+    c = Batch(lens, 2, 64, 64, dtype)
+    for copies in (1, 9):
+        table, kv = c.table.repeat(copies, 1), c.kv_lens.repeat(copies)
+        off = offsets(*(new * copies))
+        q = torch.randn(sum(new) * copies, 64, 64, generator=gen(3), device=DEV).to(dtype)
+        got = kernels.prompt_attention(q, c.k_pages, c.v_pages, table, kv, off)
+        kernels.check_device_error()
+        for i in {0, len(new) * copies - 1, 1}:
+            b, rows = i % len(new), slice(int(off[i]), int(off[i + 1]))
+            check(got[rows], *attend(q[rows], c.k[b], c.v[b], lens[b] - new[b], None, 0, 0.125, dtype))
+
+
+# ------------------------------------------------------------------ rope in runs of heads
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("f32_table", [True, False])
+@pytest.mark.parametrize("norm", [True, False])
+@pytest.mark.parametrize("nq,nkv", [(32, 8), (20, 10), (9, 9)])
+@pytest.mark.parametrize("order", ["phsd", "pshd", "both"])
+def test_rope_in_runs_of_heads(dtype, hd, f32_table, norm, nq, nkv, order):
+    """Enough tokens for runs of 8 heads, full ones and remainders; tolerances as in test_rope."""
+    lens, new = [3001, 17, 0, 2500], [2990, 17, 0, 2201]
+    T = sum(new) + 5
+    runs = -(-nq // 8) + 2 * -(-nkv // 8)
+    assert T * runs * (hd // 16) >= 256 * 2 * torch.cuda.get_device_properties(0).multi_processor_count
+    from test_paged_gpu import rope_want
+    c = Batch(lens, nkv, hd, 64, dtype, order=order)
+    g = gen(hd + nq)
+    packed = torch.randn(T, nq + 2 * nkv, hd, generator=g, device=DEV).to(dtype)
+    q, k, v = packed[:, :nq], packed[:, nq:nq + nkv], packed[:, nq + nkv:]
+    cos, sin = (torch.randn(max(lens), hd, generator=g, device=DEV).to(torch.float32 if f32_table else dtype)
+                for _ in range(2))
+    qw, kw = ((1 + 0.2 * torch.randn(hd, generator=g, device=DEV)).to(dtype) if norm else None for _ in range(2))
+    kp, vp = c.k_pages.clone(), c.v_pages.clone()
+    got = kernels.qk_norm_rope(q, k, v, cos, sin, *c.cache(), offsets(*new), q_weight=qw, k_weight=kw, eps=1e-5)
+    kernels.check_device_error()
+    h = torch.finfo(dtype).eps / 2
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    room = (hd / 2 + 32) * 2.0 ** -24
+    at = 0
+    for b, n in enumerate(new):
+        rows = slice(at, at + n)
+        at += n
+        if not n:
+            continue
+        pos = torch.arange(lens[b] - n, lens[b], device=DEV)
+        (qo, qm), (ko, km) = rope_want(q[rows], k[rows], cos, sin, pos, qw, kw, 1e-5)
+        assert ((got[rows].double() - qo).abs() <= h * qo.abs() + room * qm + tiny).all()
+        pages, slots = c.where(b, lens[b] - n, n)
+        kept = c.k_pages[pages, :, slots]
+        assert ((kept.double() - ko).abs() <= h * ko.abs() + room * km + tiny).all()
+        kp[pages, :, slots], vp[pages, :, slots] = kept, v[rows]
+    assert (got[at:] == 0).all()
+    for now, then in ((c.k_pages, kp), (c.v_pages, vp)):   # v as it was given, every other slot as it was
+        assert torch.equal(now.contiguous().view(torch.int16), then.contiguous().view(torch.int16))
+
+
+# ------------------------------------------------------------------ several host threads
+
+def test_every_result_of_several_threads():
+    """Each thread on its own stream, every one of its results compared."""
+    import threading
+    c = Batch([900, 40, 9000], 2, 128, 16, torch.float16)
+    q = torch.randn(3, 8, 128, generator=gen(2), device=DEV).half()
+    off = offsets(1, 1, 1)
+    k, v = (torch.randn(3, 2, 128, generator=gen(i), device=DEV).half() for i in (3, 4))
+    cos, sin = (torch.randn(9000, 128, generator=gen(i), device=DEV) for i in (5, 6))
+    spare = [torch.empty_like(x) for x in (c.k_pages, c.v_pages)]   # not what the attention reads
+
+    def calls(pools):
+        return (kernels.paged_attention(q, *c.cache()), kernels.prompt_attention(q, *c.cache(), off),
+                kernels.qk_norm_rope(q, k, v, cos, sin, *pools, c.table, c.kv_lens))
+
+    want = calls(spare)
+    torch.cuda.synchronize()
+    done, wrong = [], []
+
+    def work():
+        try:
+            pools = [torch.empty_like(x) for x in spare]
+            with torch.cuda.stream(torch.cuda.Stream(DEV)):
+                got = [calls(pools) for _ in range(50)]
+                torch.cuda.current_stream().synchronize()
+            done.append(sum(all(torch.equal(a, b) for a, b in zip(x, want)) for x in got))
+        except BaseException as e:   # noqa: BLE001  (an exception in a thread is a failure here)
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work) for _ in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong and done == [50] * 3
+    kernels.check_device_error()
