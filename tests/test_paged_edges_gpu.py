@@ -562,3 +562,100 @@ def test_every_result_of_several_threads():
         t.join()
     assert not wrong and done == [50] * 3
     kernels.check_device_error()
+
+
+# ------------------------------------------------------------------ lengths and batches
+
+@pytest.mark.parametrize("window,sinks", [(None, 0), (3, 0), (3, 1), (2 ** 31 - 1, 0), (2 ** 31 - 1, 2 ** 31 - 1)])
+@pytest.mark.parametrize("hd,group", [(64, 4), (128, 1)])
+def test_more_rows_than_the_length_counts(window, sinks, hd, group):
+    """Rows before the first token see nothing; the others are right; recorded."""
+    for rows, length in ((12, 5), (300, 5), (300, 290), (9, 0)):
+        c = Batch([length, 50], 1, hd, 16, torch.float16)
+        q = torch.randn(rows + 20, group, hd, generator=gen(2), device=DEV).half()
+        got = kernels.prompt_attention(q, *c.cache(), offsets(rows, 20), window=window, sinks=sinks)
+        with pytest.raises(Exception, match="out of range"):
+            kernels.check_device_error()
+        early = rows - length
+        assert (got[:early] == 0).all()
+        if length:
+            check(got[early:rows], *attend(q[early:rows], c.k[0], c.v[0], 0, window, sinks, hd ** -0.5, torch.float16))
+        check(got[rows:], *attend(q[rows:], c.k[1], c.v[1], 30, window, sinks, hd ** -0.5, torch.float16))
+
+
+@pytest.mark.parametrize("batch", [33, 70, 1025, 4000])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (20, 2)])
+def test_prompts_and_steps_of_many_sequences(batch, window, sinks):
+    """A row tile finds its sequence among thousands, many of them without a new token."""
+    g = torch.Generator().manual_seed(batch)
+    new = [int(x) if y > 0 else 0 for x, y in zip(torch.randint(1, 6, (batch,), generator=g),
+                                                 torch.randint(0, 3, (batch,), generator=g))]
+    new[batch // 2], new[batch - 1] = 150, 77
+    lens = [n + int(x) for n, x in zip(new, torch.randint(0, 40, (batch,), generator=g))]
+    hd, dtype = 64, torch.bfloat16
+    width = -(-max(lens) // 16)
+    # sequences of a batch share a few pages: enough of them to tell one from another
+    n_pages = 500
+    pools = [torch.randn(n_pages, 1, 16, hd, generator=gen(i), device=DEV).to(dtype) for i in range(2)]
+    table = torch.randint(0, n_pages, (batch, width), generator=gen(5), device=DEV, dtype=torch.int32)
+    kv = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    off = offsets(*new)
+    q = torch.randn(sum(new) + 3, 3, hd, generator=gen(7), device=DEV).to(dtype)
+    got = kernels.prompt_attention(q, *pools, table, kv, off, window=window, sinks=sinks)
+    step = torch.randn(batch, 3, hd, generator=gen(8), device=DEV).to(dtype)
+    one = kernels.paged_attention(step, *pools, table, kv, window=window, sinks=sinks)
+    kernels.check_device_error()
+    assert (got[sum(new):] == 0).all()
+    at = 0
+    for b, n in enumerate(new):
+        if batch <= 70 or b % 41 == 0 or n > 5 or b > batch - 20:
+            k, v = (x[table[b].long()].transpose(1, 2).reshape(-1, 1, hd)[:lens[b]] for x in pools)
+            if n:
+                check(got[at:at + n], *attend(q[at:at + n], k, v, lens[b] - n, window, sinks, 0.125, dtype))
+            if lens[b]:
+                check(one[b:b + 1], *attend(step[b:b + 1], k, v, lens[b] - 1, window, sinks, 0.125, dtype))
+            else:
+                assert (one[b] == 0).all()
+        at += n
+
+
+def test_a_captured_padded_batch():
+    """One graph, replayed for batches of other lengths, offsets and pages: rows behind the last
+    sequence are zero and nothing of the replay before is left."""
+    hd, rows, batch = 128, 200, 4
+    c = Batch([400, 300, 200, 100], 2, hd, 16, torch.float16)
+    wide = torch.full((batch, 2000), -9, dtype=torch.int32, device=DEV)   # a server's: far wider than needed
+    wide[:, :c.table.shape[1]] = c.table
+    packed = torch.randn(rows, 12, hd, generator=gen(2), device=DEV).half()
+    cos, sin = torch.ones(500, hd, device=DEV), torch.zeros(500, hd, device=DEV)
+    off, lens = offsets(50, 50, 50, 50), c.kv_lens.clone()
+
+    def step():
+        q, k, v = packed[:, :8], packed[:, 8:10], packed[:, 10:]
+        r = kernels.qk_norm_rope(q, k, v, cos, sin, c.k_pages, c.v_pages, wide, lens, off)
+        return r, kernels.prompt_attention(r, c.k_pages, c.v_pages, wide, lens, off, window=250, sinks=3)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        rotated, out = step()
+    for new, total in (([50, 50, 50, 50], [400, 300, 200, 100]), ([1, 0, 130, 7], [390, 0, 150, 99]),
+                       ([0, 0, 0, 0], [0, 0, 0, 0]), ([200, 0, 0, 0], [400, 12, 0, 3]), ([0, 0, 0, 1], [0, 0, 0, 1])):
+        off.copy_(offsets(*new))
+        lens.copy_(torch.tensor(total, dtype=torch.int32))
+        packed.copy_(torch.randn(rows, 12, hd, generator=gen(sum(total)), device=DEV))
+        graph.replay()
+        torch.cuda.synchronize()
+        kernels.check_device_error()
+        at = 0
+        for b, n in enumerate(new):
+            if n:
+                pages, slots = c.where(b, 0, total[b])
+                k, v = c.k_pages[pages, :, slots], c.v_pages[pages, :, slots]
+                assert torch.equal(k[total[b] - n:], packed[at:at + n, 8:10]) and torch.equal(rotated[at:at + n],
+                                                                                             packed[at:at + n, :8])
+                check(out[at:at + n], *attend(packed[at:at + n, :8], k, v, total[b] - n, 250, 3, hd ** -0.5,
+                                              torch.float16))
+            at += n
+        assert (out[at:] == 0).all() and (rotated[at:] == 0).all()
