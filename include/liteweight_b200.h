@@ -456,9 +456,11 @@ int lw_qk_norm_rope(const lw_qk_norm_rope_args* args, lw_stream_t stream);
 /* Attention over the paged cache: position p of sequence b sees key j when
  * j <= p and (window <= 0, or p - j < window, or j < sinks);
  *   out = sum_j softmax_j(scale * q.k_j) v_j,
- * zero where no key is visible. Keys outside the mask never reach a result,
- * whatever they hold. Scores, softmax and sums in fp32; the softmax weights are
- * rounded to dtype for the second product.
+ * zero where no key is visible (NaN where every visible score is minus infinity).
+ * Keys outside the mask never reach a result, whatever they hold. Scores, softmax
+ * and sums in fp32; the softmax weights are rounded to dtype for the second product
+ * (fp16 in its upper range: one is off by at most 2^-40 of the largest, in prompts
+ * 2^-32, where half a step is less).
  *
  * q_offsets NULL: one new token per sequence (tokens == batch), the cache's
  * length split over the GPU and joined; else prompt chunks. n_q_heads is a

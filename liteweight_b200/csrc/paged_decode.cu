@@ -23,9 +23,9 @@
 // Few short sequences: a cluster of up to eight CTAs takes an item and merges
 // through distributed shared memory: one launch, no workspace.
 //
-// Measured (device time): 64 sequences of 131 to 16384 tokens, 32 / 8 heads of 128,
-// 0.90 GB: 144-151 us, 6.0-6.3 TB/s; one of 131071 tokens, 0.54 GB: 90-93 us, 5.8-6.0
-// TB/s; one of 517 tokens: 5.4 us. The stream itself runs at 7.0 TB/s; the rest is
+// Measured (device time, several GPUs): 64 sequences of 131 to 16384 tokens, 32 / 8
+// heads of 128, 0.90 GB: 144-152 us, 5.9-6.3 TB/s; one of 131071 tokens, 0.54 GB: 89-95
+// us, 5.7-6.0 TB/s; one of 517 tokens: 5.4 us. The stream itself runs at 7.0 TB/s; the rest is
 // the start (3 us), SMs that end later than others, the merge and the join (5 us).
 // A warp's tile takes 0.5 us of work against 1.5 us of its share of the memory.
 //

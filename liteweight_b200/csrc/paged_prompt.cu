@@ -43,14 +43,16 @@
 //
 // Every wait is bounded; on expiry LW_ERR_TIMEOUT is recorded and the CTA ends.
 //
-// Measured (32 / 8 heads of 128): one prompt of 8192 tokens 540 us, 1.0 PFLOP/s, 0.6 of
-// the measured burst of a bf16 GEMM at an SM clock of 1.6 to 1.75 GHz under the
-// power limit; six prompts of 129 to 2111 tokens 252 us, 0.91 PFLOP/s. Per key tile
-// the tensor cores and the special-function unit (exponentials) need 2048 cycles
-// each for the two row tiles; a tile takes 3480: a row tile's softmax (2300) and
-// its way through the tensor cores (1160) follow one another. Making S before it
-// is waited for did not shorten it (526 -> 575 us): the bound is what two softmax
-// warps per scheduler get through. Four (two threads per row) were slower (685).
+// Measured (32 / 8 heads of 128; several GPUs): one prompt of 8192 tokens 547 - 566
+// us, 0.97 - 1.0 PFLOP/s, 0.6 of the measured burst of a bf16 GEMM at an SM clock of
+// 1.6 to 1.75 GHz under the power limit; six prompts of 129 to 2111 tokens 249 - 255
+// us, 0.90 - 0.92 PFLOP/s. Per key tile the tensor cores and the special-function
+// unit (exponentials) need 2048 cycles each for the two row tiles; a tile takes
+// 3480. No unit is full (tensor and special function 58 %, issue 36 %): the period is
+// a chain, a row tile's softmax (2300: read and mask 260, maximum 250, rescale check
+// 155, exponentials 1450) and then its way through the tensor cores (1160). Making S
+// before it is waited for (526 -> 575 us) and two threads per row (685) did not
+// shorten it; weights formed before the tile's maximum is known are not built.
 #include <algorithm>
 #include <cmath>
 

@@ -13,7 +13,8 @@
 //   o_hi = r (x_hi [w_hi cos_hi] + x_lo [w_lo sin_hi])
 // All of it in fp32 with one rounding at the store. Memory bound: every element
 // is read once and written once. 11064 tokens of 64 + 2x8 heads of 128 (bf16, fp32
-// tables): 76 us, 6.0 TB/s, 0.92 of a copy's rate. One token: 2.4 us, a launch.
+// tables): 76 - 78 us on several GPUs, 5.9 - 6.0 TB/s, 0.9 of a copy's rate. One token:
+// 2.4 us, a launch.
 #include "paged.cuh"
 
 namespace lw {
