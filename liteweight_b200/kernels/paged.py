@@ -123,7 +123,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
     over the keys j that position p = kv_lens[b] - 1 sees: all of 0 .. p, or with
     a window those with p - j < window or j < sinks. Query head h reads kv head
-    h // (q heads / kv heads). A sequence of length 0 gives zeros.
+    h // (q heads / kv heads). A sequence of length 0 gives zeros; one whose scores are
+    all minus infinity gives NaN. The softmax weights are rounded to q's type for the
+    product with v; scores, maxima and sums are fp32.
 
     Args:
         q:      [batch, q heads, head_dim], in the cache's dtype
@@ -146,7 +148,8 @@ def prompt_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
         q:      [tokens, q heads, head_dim], in the cache's dtype
         out:    [tokens, q heads, head_dim] (may not overlap q)
 
-    Rows from q_offsets[-1] on are zero, or left as they were in a given `out`.
+    Rows from q_offsets[-1] on, and those of a sequence whose offsets run past q (which
+    is recorded), are zero, or left as they were in a given `out`.
     """
     assert q_offsets is not None, "q_offsets: int32 [batch + 1]"
     return _attention(q, k_pages, v_pages, page_table, kv_lens, q_offsets, window, sinks, scale, out)
